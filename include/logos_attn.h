@@ -43,7 +43,9 @@ typedef enum {
     LOGOS_ERR_ALIGNMENT = 6,     /* pointer or extent breaks a 16-byte requirement   */
     LOGOS_ERR_SCRATCH_LIMIT = 7, /* request exceeds the fixed scratch of
                                     logos_decode_int8_noalloc                        */
-    LOGOS_ERR_KERNEL_TIMEOUT = 8 /* a bounded wait inside a kernel ran out           */
+    LOGOS_ERR_KERNEL_TIMEOUT = 8,/* a bounded wait inside a kernel ran out           */
+    LOGOS_ERR_BAD_BATCH = 9      /* a paged batch on the device breaks its own bounds;
+                                    reported by logos_ctx_synchronize                */
 } logos_status;
 
 typedef enum { LOGOS_F32 = 0, LOGOS_BF16 = 1, LOGOS_F16 = 2 } logos_dtype;
@@ -419,6 +421,98 @@ int logos_mha_forward_f32(logos_ctx* ctx, const float* X, const float* W_Q, cons
  * the arithmetic of the reference's vedic_gemm (include/VedicGEMM.hpp) up to the order of the additions. */
 int logos_gemm_f32(logos_ctx* ctx, const float* A, int lda, int64_t strideA, const float* B, int ldb,
                    int64_t strideB, float* C, int ldc, int64_t strideC, int M, int N, int K, int batch);
+
+/* ---- norm and position rotation of queries and keys ----------------------- */
+
+/* The preparation of queries and keys in models that normalise every head and rotate it by its position; one
+ * pass over Q and K.  The reference has neither (its positions enter through the embedding).  For a row x of one
+ * head (DH values, token at position p, weight w of Q or of K):
+ *   n_i = x_i w_i / sqrt(mean(x^2) + eps)
+ *   pair k of the first `dims` channels, (a, b) = (k, k + dims/2) or, interleaved, (2k, 2k + 1), angle p inv_freq[k]:
+ *   y_a = n_a cos - n_b sin,   y_b = n_b cos + n_a sin;   channels from `dims` on: y_i = n_i.
+ * fp32 arithmetic, one rounding at the end.  The angle is reduced exactly (position times a 64-bit fixed-point
+ * number of turns), so it is as good at position 2^31 - 1 as at 1. */
+#define LOGOS_ROPE_MAX_PAIRS 64
+typedef struct {
+    int dims;          /* rotated channels: 0 (none) ... DH, a multiple of 16 */
+    int interleaved;   /* 0: pairs (k, k + dims/2); 1: pairs (2k, 2k + 1)      */
+    double inv_freq[LOGOS_ROPE_MAX_PAIRS];   /* radians per position of pair k < dims/2; finite */
+} logos_rope;
+/* Element strides of a [rows][heads][DH] tensor whose rows are contiguous; NULL where one is taken: packed.  The
+ * head-major tensor [heads][rows][DH] of logos_qkv_project (one sequence of `rows` tokens) is {DH, rows * DH}. */
+typedef struct { int64_t row, head; } logos_row_strides;
+/* Q [rows][Hq][DH], K [rows][Hk][DH] in `dtype` (F32, BF16, FP16), DH 64 or 128; weights fp32 [DH], positions int32
+ * [rows].  A NULL weight leaves the norm of that tensor out (rotation only).  Hq or Hk may be 0, its pointers NULL.
+ * Rows and weights 16-byte aligned.  Outputs may be the inputs themselves with the same strides; any other overlap
+ * is not allowed. */
+int logos_qk_norm_rope(logos_ctx* ctx, int dtype, const void* Q, const void* K, const float* q_weight,
+                       const float* k_weight, const int32_t* positions, const logos_rope* rope, float eps, void* Q_out,
+                       void* K_out, int rows, int Hq, int Hk, int DH, const logos_row_strides* q_in,
+                       const logos_row_strides* k_in, const logos_row_strides* q_out, const logos_row_strides* k_out);
+/* Its backward pass: from the raw Q, K and the gradients of the outputs, the gradients of Q, K (in `dtype`) and of the
+ * weights (fp32 [DH], summed over rows and heads in a fixed order: reproducible bit for bit).  dQ may be dQ_out itself
+ * with the same strides (K alike).  dq_weight / dk_weight are NULL exactly where the weight is.  Workspace from the
+ * context (logos_qk_norm_rope_bwd_workspace_bytes / logos_ctx_reserve). */
+size_t logos_qk_norm_rope_bwd_workspace_bytes(int DH);
+int logos_qk_norm_rope_bwd(logos_ctx* ctx, int dtype, const void* Q, const void* K, const void* dQ_out,
+                           const void* dK_out, const float* q_weight, const float* k_weight, const int32_t* positions,
+                           const logos_rope* rope, float eps, void* dQ, void* dK, float* dq_weight, float* dk_weight,
+                           int rows, int Hq, int Hk, int DH, const logos_row_strides* q_in,
+                           const logos_row_strides* k_in, const logos_row_strides* dq_out,
+                           const logos_row_strides* dk_out, const logos_row_strides* dq, const logos_row_strides* dk);
+
+/* ---- paged INT8 KV cache ---------------------------------------------------- */
+
+/* The Nikhilam quantiser with one scale per (token, head) row, scale = (max|x| + 1e-8) / 127.5, q = round-half-even
+ * of x / scale held to +-127 (the arithmetic of nikhilam_compress, cuda/ModelGPU.cu:357-386, applied to a row), in
+ * pages that sequences of any length take from one pool.  A row is quantised once, when it is written, whatever comes
+ * later.  One layer's pages: */
+typedef struct {
+    int8_t *k, *v;               /* [pages][H][page_size][DH], 16-byte aligned      */
+    float *k_scale, *v_scale;    /* [pages][H][page_size], 16-byte aligned          */
+    int pages, page_size;        /* page_size 16, 32, 64 or 128                     */
+    int H, DH;                   /* key/value heads; DH 64 or 128                   */
+} logos_paged_cache;
+/* The new tokens of a batch of sequences.  Sequence b owns rows [cu_q[b], cu_q[b+1]) of the token tensors; they stand
+ * at positions kv_len[b] - n ... kv_len[b] - 1 (n of them); position p lives in row p % page_size of page
+ * page_table[b][p / page_size].  Rows from cu_q[B] on are neither read nor written.  The three tables are device
+ * memory, so that a captured graph replays with new contents; B, rows, max_q and max_kv are host-side bounds that
+ * size the launches.  Sequences may share pages that none of them writes in the call; a page row that two sequences
+ * write in one call holds the row of either or a mixture of both.
+ * The kernels check what they read from the tables: a sequence that breaks a bound (0 <= n <= max_q, n <= kv_len <=
+ * max_kv, its rows inside `rows`) is left out, a page outside the cache is skipped, no access leaves the tensors,
+ * and the next logos_ctx_synchronize returns LOGOS_ERR_BAD_BATCH. */
+typedef struct {
+    const int32_t* cu_q;         /* [B + 1], cu_q[0] = 0, not falling               */
+    const int32_t* kv_len;       /* [B]: tokens of the sequence, the new ones included */
+    const int32_t* page_table;   /* [B][max_pages]; entries behind the last page in use are not read */
+    int B, max_pages;
+    int rows;                    /* rows of the token tensors, at least cu_q[B]     */
+    int max_q, max_kv;           /* bounds of a sequence's new tokens and of kv_len; max_kv <= max_pages * page_size */
+} logos_paged_batch;
+
+/* Quantises the new tokens' K and V ([rows][H][DH] in `dtype`, F32, BF16 or FP16; strides or NULL) into their pages. */
+int logos_paged_append(logos_ctx* ctx, int dtype, const void* K, const void* V, const logos_row_strides* k_in,
+                       const logos_row_strides* v_in, const logos_paged_cache* cache, const logos_paged_batch* batch);
+/* The inverse: the values (float)q * scale that the cache holds for the batch's rows, in `dtype`.  cu_q over whole
+ * sequences (n = kv_len) reads all of them out. */
+int logos_paged_read(logos_ctx* ctx, int dtype, const logos_paged_cache* cache, const logos_paged_batch* batch, void* K,
+                     void* V, const logos_row_strides* k_out, const logos_row_strides* v_out);
+/* Attention of the batch's new tokens -- one per sequence, a chunk of a prompt, or both kinds in one call -- over the
+ * pages, whose rows must have been written (logos_paged_append): Q and O [rows][Hq][DH] in `dtype` (BF16, FP16), query
+ * head h reads key/value head h / (Hq / H); Hq a multiple of H.  A token at position i sees the positions j < kv_len of
+ * its sequence that `params` allows: j <= i when causal, and the Shunyam rule (window, stride) in a sequence longer
+ * than the window.  The Navier-Stokes terms are not offered here (LOGOS_ERR_UNSUPPORTED: apply the advection to
+ * Q and the diffusion to V before they get here); scale > 0.  A row that sees nothing gets zeros.
+ * The int8 values enter the products exactly, the scales stay fp32; weights are rounded to FP16 once, sums are fp32.
+ * Results do not depend on what else is in the batch beyond the split of the keys, which the bounds decide;
+ * the same call gives the same bits.  O may not overlap Q.  Workspace from the context
+ * (logos_paged_attention_workspace_bytes / logos_ctx_reserve); calls that share a context run one after the other. */
+size_t logos_paged_attention_workspace_bytes(logos_ctx* ctx, const logos_paged_cache* cache,
+                                             const logos_paged_batch* batch, int Hq);
+int logos_paged_attention(logos_ctx* ctx, int dtype, const void* Q, const logos_paged_cache* cache,
+                          const logos_paged_batch* batch, int Hq, const logos_attn_params* params, void* O,
+                          const logos_row_strides* q_in, const logos_row_strides* o_out);
 
 /* ---- heads over several GPUs -------------------------------------------- */
 

@@ -85,6 +85,7 @@ const char* logos_status_string(int status) {
         case LOGOS_ERR_NO_DEVICE: return "no sm_100 CUDA device";
         case LOGOS_ERR_ALIGNMENT: return "misaligned pointer or extent";
         case LOGOS_ERR_KERNEL_TIMEOUT: return "a bounded wait inside a kernel ran out";
+        case LOGOS_ERR_BAD_BATCH: return "a paged batch breaks its bounds or names a page outside the cache";
         case LOGOS_ERR_SCRATCH_LIMIT: return "request exceeds the fixed scratch of the no-allocation entry point";
     }
     return "unknown status";
@@ -206,6 +207,10 @@ int logos_ctx_synchronize(logos_ctx* ctx) {
     LOGOS_CUDA_TRY(ctx, cudaMemcpy(&flag, ctx->tc_status, sizeof(int), cudaMemcpyDeviceToHost));
     if (flag) {
         cudaMemset(ctx->tc_status, 0, sizeof(int));
+        if (flag & logos::kBadBatchFlag)
+            return logos::fail(ctx, LOGOS_ERR_BAD_BATCH,
+                               "sequence %d of a paged batch: %s; what a call left out is not defined", flag & 0xffffff,
+                               (flag & 0x01000000) ? "a page outside the cache" : "row range, new tokens or kv_len outside the batch's bounds");
         if (flag & 0x20000000)
             return logos::fail(ctx, LOGOS_ERR_KERNEL_TIMEOUT,
                                "rank %d of the comm did not deliver its rows within %d ms; the gathered output is invalid",
@@ -318,6 +323,61 @@ int logos_attention_fwd_strided(logos_ctx* ctx, int in_dtype, int out_dtype, con
     if (!strided && !ctx->force_general && logos::attention_window_eligible(in_dtype, out_dtype, DH, params, S))
         return logos::attention_window(ctx, in_dtype, out_dtype, Q, K, V, O, B, H, S, DH, params);
     return logos::attention_simt(ctx, in_dtype, out_dtype, Q, K, V, O, B, H, S, DH, params, qkv, out);
+}
+
+int logos_qk_norm_rope(logos_ctx* ctx, int dtype, const void* Q, const void* K, const float* q_weight,
+                       const float* k_weight, const int32_t* positions, const logos_rope* rope, float eps, void* Q_out,
+                       void* K_out, int rows, int Hq, int Hk, int DH, const logos_row_strides* q_in,
+                       const logos_row_strides* k_in, const logos_row_strides* q_out, const logos_row_strides* k_out) {
+    if (!ctx) return LOGOS_ERR_INVALID_ARG;
+    logos::DeviceScope on(ctx);
+    return logos::qk_norm_rope(ctx, dtype, false, Q, K, nullptr, nullptr, q_weight, k_weight, positions, rope, eps, Q_out,
+                               K_out, nullptr, nullptr, rows, Hq, Hk, DH, q_in, k_in, nullptr, nullptr, q_out, k_out);
+}
+
+size_t logos_qk_norm_rope_bwd_workspace_bytes(int DH) { return DH > 0 ? logos::qk_norm_rope_bwd_workspace_bytes(DH) : 0; }
+
+int logos_qk_norm_rope_bwd(logos_ctx* ctx, int dtype, const void* Q, const void* K, const void* dQ_out,
+                           const void* dK_out, const float* q_weight, const float* k_weight, const int32_t* positions,
+                           const logos_rope* rope, float eps, void* dQ, void* dK, float* dq_weight, float* dk_weight,
+                           int rows, int Hq, int Hk, int DH, const logos_row_strides* q_in,
+                           const logos_row_strides* k_in, const logos_row_strides* dq_out,
+                           const logos_row_strides* dk_out, const logos_row_strides* dq, const logos_row_strides* dk) {
+    if (!ctx) return LOGOS_ERR_INVALID_ARG;
+    logos::DeviceScope on(ctx);
+    return logos::qk_norm_rope(ctx, dtype, true, Q, K, dQ_out, dK_out, q_weight, k_weight, positions, rope, eps, dQ, dK,
+                               dq_weight, dk_weight, rows, Hq, Hk, DH, q_in, k_in, dq_out, dk_out, dq, dk);
+}
+
+int logos_paged_append(logos_ctx* ctx, int dtype, const void* K, const void* V, const logos_row_strides* k_in,
+                       const logos_row_strides* v_in, const logos_paged_cache* cache, const logos_paged_batch* batch) {
+    if (!ctx) return LOGOS_ERR_INVALID_ARG;
+    logos::DeviceScope on(ctx);
+    return logos::paged_append(ctx, dtype, K, V, k_in, v_in, cache, batch);
+}
+
+int logos_paged_read(logos_ctx* ctx, int dtype, const logos_paged_cache* cache, const logos_paged_batch* batch, void* K,
+                     void* V, const logos_row_strides* k_out, const logos_row_strides* v_out) {
+    if (!ctx) return LOGOS_ERR_INVALID_ARG;
+    logos::DeviceScope on(ctx);
+    return logos::paged_read(ctx, dtype, cache, batch, K, V, k_out, v_out);
+}
+
+size_t logos_paged_attention_workspace_bytes(logos_ctx* ctx, const logos_paged_cache* cache,
+                                             const logos_paged_batch* batch, int Hq) {
+    if (!ctx || !cache || !batch || logos::paged_check(ctx, "paged_attention", cache, batch) != LOGOS_OK || Hq <= 0 ||
+        Hq % cache->H)
+        return 0;
+    return logos::paged_attention_workspace_bytes(ctx, cache, batch, Hq);
+}
+
+int logos_paged_attention(logos_ctx* ctx, int dtype, const void* Q, const logos_paged_cache* cache,
+                          const logos_paged_batch* batch, int Hq, const logos_attn_params* params, void* O,
+                          const logos_row_strides* q_in, const logos_row_strides* o_out) {
+    if (!ctx) return LOGOS_ERR_INVALID_ARG;
+    if (!params_ok(params)) return logos::fail(ctx, LOGOS_ERR_INVALID_ARG, "paged_attention: bad parameter block");
+    logos::DeviceScope on(ctx);
+    return logos::paged_attention(ctx, dtype, Q, cache, batch, Hq, params, O, q_in, o_out);
 }
 
 size_t logos_attention_bwd_workspace_bytes(int B, int H, int S, int DH) {

@@ -142,6 +142,26 @@ inline cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, dim3 b
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// Makes the context's device current for the length of a call (the stream, the launches and the attributes belong
+// to it, whatever device the caller has current) and puts the caller's back.
+struct DeviceScope {
+    int before = -1;
+    explicit DeviceScope(const logos_ctx* ctx) {
+        if (cudaGetDevice(&before) != cudaSuccess || before == ctx->device) before = -1;
+        else cudaSetDevice(ctx->device);
+    }
+    ~DeviceScope() { if (before >= 0) cudaSetDevice(before); }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
+// what a kernel writes to logos_ctx::tc_status when a paged batch is not what its bounds say: this flag, the
+// sequence in the low 24 bits, bit 24 set for a page outside the cache
+constexpr int kBadBatchFlag = 0x10000000, kBadPageBit = 0x01000000;
+__device__ __forceinline__ void report_batch(int* status, int sequence, bool page) {
+    atomicCAS(status, 0, kBadBatchFlag | (page ? kBadPageBit : 0) | (sequence & 0xffffff));
+}
+
 // The first 64 KiB of a context's workspace are the split-K arrival counters of the decode kernel.  They are
 // zero whenever no decode kernel is running (cleared when the block is attached, put back to zero by the
 // kernel itself); every other user of the workspace starts beyond them.
@@ -149,6 +169,17 @@ constexpr size_t kWorkspaceCounterBytes = 64 * 1024;
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
+
+// strides of a [rows][heads][DH] tensor: every row on a 16-byte boundary; no two rows on one another (an output)
+inline bool rows_aligned(const logos_row_strides& s, size_t esz) {
+    return s.row >= 0 && s.head >= 0 && (s.row * esz) % 16 == 0 && (s.head * esz) % 16 == 0;
+}
+inline bool rows_apart(const logos_row_strides& s, int64_t rows, int64_t heads, int DH) {
+    if (heads <= 0) return true;
+    if (rows <= 1) return heads <= 1 || s.head >= DH;
+    if (heads <= 1) return s.row >= DH;
+    return (s.head >= DH && s.row >= (heads - 1) * s.head + DH) || (s.row >= DH && s.head >= (rows - 1) * s.row + DH);
+}
 
 inline size_t dtype_size(int dt) { return dt == LOGOS_F32 ? 4 : 2; }
 inline bool dtype_ok(int dt) { return dt == LOGOS_F32 || dt == LOGOS_BF16 || dt == LOGOS_F16; }
@@ -230,6 +261,21 @@ int decode_int8(logos_ctx*, const void*, const void*, const int8_t*, const int8_
 // true when decode_int8 takes the new token's rows itself (append_k / append_v): the window kernel at DH = 64
 bool decode_appends_itself(const logos_attn_params* p, int DH);
 size_t decode_workspace_bytes(int B, int H, int S_max, int DH);
+int qk_norm_rope(logos_ctx*, int dtype, bool bwd, const void* Q, const void* K, const void* GQ, const void* GK,
+                 const float* wq, const float* wk, const int32_t* positions, const logos_rope*, float eps, void* YQ,
+                 void* YK, float* dwq, float* dwk, int rows, int Hq, int Hk, int DH, const logos_row_strides* q_in,
+                 const logos_row_strides* k_in, const logos_row_strides* gq_in, const logos_row_strides* gk_in,
+                 const logos_row_strides* q_out, const logos_row_strides* k_out);
+size_t qk_norm_rope_bwd_workspace_bytes(int DH);
+// argument checks shared by the paged entry points; an empty batch (no rows) is fine
+int paged_check(logos_ctx*, const char* what, const logos_paged_cache*, const logos_paged_batch*);
+int paged_append(logos_ctx*, int dtype, const void* K, const void* V, const logos_row_strides*, const logos_row_strides*,
+                 const logos_paged_cache*, const logos_paged_batch*);
+int paged_read(logos_ctx*, int dtype, const logos_paged_cache*, const logos_paged_batch*, void* K, void* V,
+               const logos_row_strides*, const logos_row_strides*);
+size_t paged_attention_workspace_bytes(logos_ctx*, const logos_paged_cache*, const logos_paged_batch*, int Hq);
+int paged_attention(logos_ctx*, int dtype, const void* Q, const logos_paged_cache*, const logos_paged_batch*, int Hq,
+                    const logos_attn_params*, void* O, const logos_row_strides*, const logos_row_strides*);
 int layer_norm(logos_ctx*, int dtype, const void* X, const float* gamma, const float* beta, void* Y, int rows, int D,
                float eps);
 int attention_simt(logos_ctx*, int in_dtype, int out_dtype, const void* Q, const void* K,

@@ -1,0 +1,477 @@
+// paged_attn.cu -- attention of new tokens over the paged INT8 cache (logos_paged_attention): the kernel for few query
+// rows per key/value head (single tokens, speculative steps, short chunks), and the dispatch.
+//
+// Mathematics.  With K_j = ks_j k8_j and V_j = vs_j v8_j (int8 rows, one fp32 scale each) and a query row q,
+//   x_j = (q . k8_j) scale log2(e) ks_j + log2(vs_j),   m = max x_j,   p_j = 2^(x_j - m),
+//   O = sum_j p_j v8_j,   l = sum_j p_j / vs_j,   o = O / l:
+// the scale of V rides in the exponent, so a weight p_j <= 1 meets plain integers, and both products run on FP16
+// operands that hold the cache's bytes exactly.  q is brought into FP16 by a power of two per row (a BF16 value fits
+// FP16's mantissa; the row's largest value becomes 2^13 ... 2^14, so only values 2^-27 below it lose bits).  p is
+// rounded to FP16 once (2^-11 relative); everything else is fp32.
+//
+// What bounds it: HBM, 2 DH + 8 bytes per cached token and head.  Both contractions sit on mma.sync m16n8k16, whose
+// fragments come straight from global memory: S = q K^T has the rows as M and the keys as N, O^T = V^T p has the
+// channels as M and the rows as N, and the accumulator of the first is the B operand of the second as it is, so p
+// never moves between threads.  The order of the channels inside a product is free, so a thread's share of a K row is
+// 16 consecutive bytes and its share of a V row DH / 8: every load is a wide one and nothing is staged in shared
+// memory.  (tcgen05 needs 128 rows to be busy and its operands in shared memory; here a head has 1 to 16.)
+// int8 -> FP16 costs five instructions for four values: bytes biased to unsigned, spliced under the exponent of 1024
+// and the bias subtracted.
+//
+// A CTA takes one sequence, head, tile of 8 or 16 rows and one chunk of the keys; its four warps take the chunk's
+// blocks in turn, each with its own running maximum, and join in shared memory.  Chunks join through the workspace:
+// the last CTA to arrive sums the partial results in the order of the chunks.
+#include "paged.cuh"
+
+namespace logos {
+namespace {
+
+constexpr int kSplitWarps = 4;
+constexpr int kSplitThreads = 32 * kSplitWarps;
+constexpr int kSpan = 2048;                      // keys whose pages a warp's lanes hold, one 16-key block each
+constexpr float kMoveMax = 8.0f;                 // log2 units by which a row may outgrow its reference maximum
+constexpr int kSplitCounters = (int)(kWorkspaceCounterBytes / sizeof(int));
+
+struct SplitArgs {
+    PagedArgs p;
+    const void* q;
+    void* o;
+    long long q_row, q_head, o_row, o_head;
+    float c;                                     // scale * log2(e)
+    int G, is_f16, causal, window, stride;
+    int chunk, splits, tiles;                    // keys per chunk; most chunks and row tiles of a (sequence, head)
+    float* part;                                 // [(sequence, head, tile)][splits][rows][DH + 2]
+    int* counters;
+};
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+    return r;
+}
+// two biased bytes (b + 128) under the exponent of 1024, minus 1152
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t biased, uint32_t sel) {
+    const uint32_t w = prmt(biased, 0x64646464u, sel), bias = 0x64806480u;
+    __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <int D>
+__device__ __forceinline__ void store_out(const SplitArgs& a, int token, int head, int d, float x, float y) {
+    const long long at = (long long)token * a.o_row + (long long)head * a.o_head + d;
+    if (a.is_f16) *reinterpret_cast<__half2*>(static_cast<__half*>(a.o) + at) = __floats2half2_rn(x, y);
+    else *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.o) + at) = __floats2bfloat162_rn(x, y);
+}
+
+// NQ: groups of 8 query rows in the tile
+template <int D, int NQ>
+__global__ void __launch_bounds__(kSplitThreads)
+paged_split_kernel(const __grid_constant__ SplitArgs a) {
+    constexpr int ROWS = 8 * NQ, KB = 2048 / D;  // keys of a block: 2 KiB of K and 2 KiB of V in a warp's registers
+    constexpr int KG = KB / 8, KS = D / 16, MT = D / 16, VW = D / 32;   // key groups; k steps of S; channel tiles; words of a V share
+    constexpr int PITCH = D + 4;
+    __shared__ float s_o[kSplitWarps][ROWS][PITCH];
+    __shared__ float s_m[kSplitWarps][ROWS], s_l[kSplitWarps][ROWS];
+    __shared__ int s_last;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int b = blockIdx.y;
+    int x = blockIdx.x;
+    const int split = x % a.splits;
+    x /= a.splits;
+    const int h = x % a.p.H, tile = x / a.p.H;
+    const PagedSeq s = paged_seq(a.p, b);
+    if (!s.ok) {
+        if (tid == 0 && blockIdx.x == 0) report_batch(a.p.status, b, false);
+        return;
+    }
+    const int r0 = tile * ROWS, n_rows = min(ROWS, s.n * a.G - r0);
+    if (n_rows <= 0) return;
+    const int first = s.kv - s.n + r0 / a.G, last = s.kv - s.n + (r0 + n_rows - 1) / a.G;   // positions of the tile's rows
+    const bool shun = shunyam_active(a.window, s.kv);
+    const bool pure = shun && a.stride <= 0;     // a window without landmarks bounds the keys on both sides
+    const int k_end = (a.causal || pure) ? last + 1 : s.kv;
+    const int k_begin = pure ? (max(0, first - a.window) & ~(KB - 1)) : 0;
+    const int n_splits = (k_end - k_begin + a.chunk - 1) / a.chunk;
+    if (split >= n_splits) return;
+    const int c0 = k_begin + split * a.chunk, c1 = min(c0 + a.chunk, k_end);
+
+    // The chunk is walked in spans of 2048 keys.  Block i of a warp in a span is keys s0 + (4 i + warp) KB ...; lane
+    // SUB i + j holds the page of its j-th 16 keys (a page never ends inside 16 keys).
+    int s0 = c0, s1 = c0, n_iter = 0, my_page = -1;
+    auto open_span = [&](int at0) {
+        constexpr int SUB = KB / 16;
+        s0 = at0;
+        s1 = min(s0 + kSpan, c1);
+        n_iter = (s1 - s0 - warp * KB + kSplitWarps * KB - 1) / (kSplitWarps * KB);
+        const int at = s0 + ((lane / SUB) * kSplitWarps + warp) * KB + (lane % SUB) * 16;
+        my_page = -1;
+        if (at < s1) {
+            my_page = paged_page(a.p, b, at);
+            if (my_page < 0) report_batch(a.p.status, b, true);
+        }
+    };
+    open_span(c0);
+
+    uint4 kr[KG][D / 64];
+    uint32_t vr[KB / 4][VW];
+    float2 ksr[KG], vsr[KG];
+    auto load_k = [&](int it) {
+#pragma unroll
+        for (int u = 0; u < KG; ++u) {
+            const int page = __shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + (u >> 1)) & 31);
+            const int key = s0 + (it * kSplitWarps + warp) * KB + 8 * u;
+            const bool in = page >= 0 && it < n_iter;
+            const size_t row = paged_row(a.p, in ? page : 0, h) + (key & ((1 << a.p.page_shift) - 1));
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i)
+                kr[u][i] = in ? __ldg(reinterpret_cast<const uint4*>(a.p.k + (row + g) * D + 64 * i + 16 * t)) : make_uint4(0, 0, 0, 0);
+            ksr[u] = in ? __ldg(reinterpret_cast<const float2*>(a.p.ks + row + 2 * t)) : make_float2(0.0f, 0.0f);
+            vsr[u] = in ? __ldg(reinterpret_cast<const float2*>(a.p.vs + row + 2 * t)) : make_float2(1.0f, 1.0f);
+        }
+    };
+    auto load_v = [&](int it) {
+#pragma unroll
+        for (int u = 0; u < KG; ++u) {
+            const int page = __shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + (u >> 1)) & 31);
+            const int key = s0 + (it * kSplitWarps + warp) * KB + 8 * u;
+            const bool in = page >= 0 && it < n_iter;
+            const size_t row = paged_row(a.p, in ? page : 0, h) + (key & ((1 << a.p.page_shift) - 1)) + 2 * t;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int8_t* at = a.p.v + (row + i) * D + g * (D / 8);
+                if (D == 64) {
+                    const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
+                    vr[2 * u + i][0] = w.x; vr[2 * u + i][1] = w.y;
+                } else {
+                    const uint4 w = in ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0, 0, 0, 0);
+                    vr[2 * u + i][0] = w.x; vr[2 * u + i][1] = w.y; vr[2 * u + i][VW - 2] = w.z; vr[2 * u + i][VW - 1] = w.w;
+                }
+            }
+        }
+    };
+    load_k(0);
+    load_v(0);
+
+    // the rows' A fragments: k step 4 i + e of the products holds channels 64 i + 16 t + 4 e ... + 3 of this thread
+    uint32_t qa[KS][4];
+    float alpha[NQ];                             // scale log2(e), with the row's power of two taken out again
+    int pos[NQ];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        if (n >= NQ) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) qa[ks][1] = qa[ks][3] = 0;
+            break;
+        }
+        const int r = 8 * n + g;
+        const bool in = r < n_rows;
+        const int token = (r0 + (in ? r : 0)) / a.G, head = h * a.G + (r0 + (in ? r : 0)) % a.G;
+        pos[n] = s.kv - s.n + token;
+        float f[D / 4];
+        const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(s.q0 + token) * a.q_row + (long long)head * a.q_head + 16 * t;
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const uint4 w = in ? *reinterpret_cast<const uint4*>(src + 64 * (i >> 1) + 8 * (i & 1)) : make_uint4(0, 0, 0, 0);
+            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float2 v;
+                if (a.is_f16) v = __half22float2(*reinterpret_cast<const __half2*>(&ww[e]));
+                else v = make_float2(__uint_as_float(ww[e] << 16), __uint_as_float(ww[e] & 0xffff0000u));
+                f[8 * i + 2 * e] = v.x;
+                f[8 * i + 2 * e + 1] = v.y;
+                top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+            }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int be = (int)(__float_as_uint(top) >> 23);
+        const int up = (be == 0 || be == 255) ? 127 : min(max(267 - be, 1), 253);   // biased exponent of the power of two
+        const float mul = __uint_as_float((uint32_t)up << 23);
+        alpha[n] = a.c * __uint_as_float((uint32_t)(254 - up) << 23);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const __half2 lo = __floats2half2_rn(f[4 * ks] * mul, f[4 * ks + 1] * mul), hi = __floats2half2_rn(f[4 * ks + 2] * mul, f[4 * ks + 3] * mul);
+            qa[ks][n] = *reinterpret_cast<const uint32_t*>(&lo);
+            qa[ks][2 + n] = *reinterpret_cast<const uint32_t*>(&hi);
+        }
+    }
+
+    float o[NQ][MT][4];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
+    }
+
+    for (;;) {
+    for (int it = 0; it < n_iter; ++it) {
+        const int k0 = s0 + (it * kSplitWarps + warp) * KB;
+        float sc[KG][4];
+        float2 inv[KG];
+        bool whole = true;                       // every key of the block is there
+#pragma unroll
+        for (int u = 0; u < KG; ++u) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[u][e] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                const uint32_t w[4] = {kr[u][i].x ^ 0x80808080u, kr[u][i].y ^ 0x80808080u, kr[u][i].z ^ 0x80808080u, kr[u][i].w ^ 0x80808080u};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mma_f16(sc[u], qa[4 * i + e], bytes_to_half2(w[e], 0x4140), bytes_to_half2(w[e], 0x4342));
+            }
+            const float v0 = fmaxf(vsr[u].x, 1e-30f), v1 = fmaxf(vsr[u].y, 1e-30f);
+            const float b0 = __log2f(v0), b1 = __log2f(v1);
+            inv[u] = make_float2(__fdividef(1.0f, v0), __fdividef(1.0f, v1));
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                sc[u][2 * n] = fmaf(sc[u][2 * n], alpha[n] * ksr[u].x, b0);
+                sc[u][2 * n + 1] = fmaf(sc[u][2 * n + 1], alpha[n] * ksr[u].y, b1);
+            }
+            whole = whole && __shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + (u >> 1)) & 31) >= 0;
+        }
+        load_k(it + 1);
+        if (!whole || shun || k0 + KB > c1 || (a.causal && k0 + KB - 1 > first)) {
+#pragma unroll
+            for (int u = 0; u < KG; ++u) {
+                const bool there = __shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + (u >> 1)) & 31) >= 0;
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = k0 + 8 * u + 2 * t + e;
+                        if (!there || key >= c1 || !key_allowed(pos[n], key, a.causal != 0, shun, a.window, a.stride)) sc[u][2 * n + e] = -INFINITY;
+                    }
+            }
+        }
+        float f[NQ];
+        bool moved = false;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float top = fmaxf(sc[0][2 * n], sc[0][2 * n + 1]);
+#pragma unroll
+            for (int u = 1; u < KG; ++u) top = fmaxf(top, fmaxf(sc[u][2 * n], sc[u][2 * n + 1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // the reference maximum moves only when a weight would pass 2^8 (well inside FP16), or at the first key
+            const bool move = top > m[n] + kMoveMax || (m[n] == -INFINITY && top > -INFINITY);
+            f[n] = (move && m[n] > -INFINITY) ? exp2_fast(m[n] - top) : 1.0f;
+            moved |= move && m[n] > -INFINITY;
+            if (move) m[n] = top;
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                l[n] *= f[n];
+                const float f0 = __shfl_sync(0xffffffffu, f[n], 8 * t), f1 = __shfl_sync(0xffffffffu, f[n], 8 * t + 4);   // rows 2t, 2t + 1
+#pragma unroll
+                for (int i = 0; i < MT; ++i) { o[n][i][0] *= f0; o[n][i][1] *= f1; o[n][i][2] *= f0; o[n][i][3] *= f1; }
+            }
+        }
+        uint32_t pb[NQ][KG];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            const float ref = m[n] == -INFINITY ? 0.0f : m[n];
+#pragma unroll
+            for (int u = 0; u < KG; ++u) {
+                const float p0 = exp2_fast(sc[u][2 * n] - ref), p1 = exp2_fast(sc[u][2 * n + 1] - ref);
+                l[n] = fmaf(p0, inv[u].x, l[n]);
+                l[n] = fmaf(p1, inv[u].y, l[n]);
+                const __half2 w = __floats2half2_rn(p0, p1);
+                pb[n][u] = *reinterpret_cast<const uint32_t*>(&w);
+            }
+        }
+        // O^T += V^T p: the thread's channels are g DH / 8 + 2 tile, + 1
+#pragma unroll
+        for (int u2 = 0; u2 < KG / 2; ++u2)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+                const uint32_t x0 = vr[4 * u2][w] ^ 0x80808080u, x1 = vr[4 * u2 + 1][w] ^ 0x80808080u;
+                const uint32_t y0 = vr[4 * u2 + 2][w] ^ 0x80808080u, y1 = vr[4 * u2 + 3][w] ^ 0x80808080u;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t mx = prmt(x0, x1, half ? 0x7362 : 0x5140), my = prmt(y0, y1, half ? 0x7362 : 0x5140);
+                    const uint32_t va[4] = {bytes_to_half2(mx, 0x4140), bytes_to_half2(mx, 0x4342),
+                                            bytes_to_half2(my, 0x4140), bytes_to_half2(my, 0x4342)};
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) mma_f16(o[n][2 * w + half], va, pb[n][2 * u2], pb[n][2 * u2 + 1]);
+                }
+            }
+        load_v(it + 1);
+    }
+    if (s1 >= c1) break;
+    open_span(s1);
+    load_k(0);
+    load_v(0);
+    }
+
+    // join the warps: statistics of row 8 n + g, then the outputs scaled to the CTA's maximum
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+        if (m[n] == -INFINITY && !(l[n] == 0.0f)) m[n] = 0.0f;   // scores that are all NaN: not an empty row
+        if (t == 0) { s_m[warp][8 * n + g] = m[n]; s_l[warp][8 * n + g] = l[n]; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = 8 * n + 2 * t + e;
+            float top = s_m[0][r];
+#pragma unroll
+            for (int w = 1; w < kSplitWarps; ++w) top = fmaxf(top, s_m[w][r]);
+            const float mine = s_m[warp][r];
+            const float f = mine == -INFINITY ? 0.0f : exp2_fast(mine - top);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                s_o[warp][r][g * (D / 8) + 2 * i] = o[n][i][e] * f;
+                s_o[warp][r][g * (D / 8) + 2 * i + 1] = o[n][i][2 + e] * f;
+            }
+        }
+    __syncthreads();
+    const size_t unit = ((size_t)b * a.p.H + h) * a.tiles + tile;
+    float* part = a.part + unit * a.splits * ROWS * (D + 2);
+    for (int i = tid; i < n_rows * (D / 2); i += kSplitThreads) {
+        const int r = i / (D / 2), d = 2 * (i % (D / 2));
+        float top = s_m[0][r], sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
+#pragma unroll
+        for (int w = 1; w < kSplitWarps; ++w) top = fmaxf(top, s_m[w][r]);
+#pragma unroll
+        for (int w = 0; w < kSplitWarps; ++w) {
+            if (s_m[w][r] == -INFINITY) continue;
+            sum = fmaf(s_l[w][r], exp2_fast(s_m[w][r] - top), sum);
+            x0 += s_o[w][r][d];
+            x1 += s_o[w][r][d + 1];
+        }
+        if (n_splits == 1) {
+            const float n = top == -INFINITY ? 0.0f : 1.0f / sum;
+            store_out<D>(a, s.q0 + (r0 + r) / a.G, h * a.G + (r0 + r) % a.G, d, x0 * n, x1 * n);
+        } else {
+            float* rec = part + ((size_t)split * ROWS + r) * (D + 2);
+            *reinterpret_cast<float2*>(rec + 2 + d) = make_float2(x0, x1);
+            if (d == 0) *reinterpret_cast<float2*>(rec) = make_float2(top, sum);
+        }
+    }
+    if (n_splits == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) s_last = atomicAdd(a.counters + unit, 1) == n_splits - 1;
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    if (tid == 0) a.counters[unit] = 0;          // as the next launch expects it
+    for (int i = tid; i < n_rows * (D / 2); i += kSplitThreads) {
+        const int r = i / (D / 2), d = 2 * (i % (D / 2));
+        const float* rec = part + (size_t)r * (D + 2);
+        float top = -INFINITY, sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
+        for (int sp = 0; sp < n_splits; ++sp) top = fmaxf(top, __ldcg(rec + (size_t)sp * ROWS * (D + 2)));
+        for (int sp = 0; sp < n_splits; ++sp) {
+            const float2 st = __ldcg(reinterpret_cast<const float2*>(rec + (size_t)sp * ROWS * (D + 2)));
+            const float2 v = __ldcg(reinterpret_cast<const float2*>(rec + (size_t)sp * ROWS * (D + 2) + 2 + d));
+            if (st.x == -INFINITY) continue;
+            const float f = exp2_fast(st.x - top);
+            sum = fmaf(st.y, f, sum);
+            x0 = fmaf(v.x, f, x0);
+            x1 = fmaf(v.y, f, x1);
+        }
+        const float n = top == -INFINITY ? 0.0f : 1.0f / sum;
+        store_out<D>(a, s.q0 + (r0 + r) / a.G, h * a.G + (r0 + r) % a.G, d, x0 * n, x1 * n);
+    }
+}
+
+// how a batch is cut: row tiles of 8 or 16, chunks of keys
+struct SplitPlan { int rows, tiles, chunk, splits; size_t bytes; };
+SplitPlan plan_split(const logos_ctx* ctx, const logos_paged_cache* c, const logos_paged_batch* b, int G) {
+    SplitPlan p;
+    const int64_t most = (int64_t)b->max_q * G;              // query rows of a (sequence, head)
+    p.rows = most <= 8 ? 8 : 16;
+    p.tiles = (int)((most + p.rows - 1) / p.rows);
+    const int64_t units = (int64_t)b->B * c->H * p.tiles;
+    // enough chunks for four CTAs on every SM, none shorter than 128 keys (a block per warp at DH 64)
+    const int64_t want = (4LL * ctx->sm_count + units - 1) / (units > 0 ? units : 1);
+    int64_t chunk = (b->max_kv + want - 1) / want;
+    chunk = chunk > kSpan && units <= kSplitCounters ? kSpan : chunk;
+    if (units > kSplitCounters) chunk = b->max_kv;           // no counters to join chunks with, and CTAs enough
+    chunk = (chunk + 127) / 128 * 128;
+    p.chunk = chunk < 128 ? 128 : (int)chunk;
+    p.splits = (b->max_kv + p.chunk - 1) / p.chunk;
+    p.bytes = kWorkspaceCounterBytes + (size_t)units * p.splits * p.rows * (c->DH + 2) * sizeof(float);
+    return p;
+}
+
+template <int D>
+int launch_split(logos_ctx* ctx, const SplitArgs& a, int rows) {
+    const dim3 grid((unsigned)((int64_t)a.splits * a.p.H * a.tiles), a.p.B);
+    if (rows == 8) paged_split_kernel<D, 1><<<grid, kSplitThreads, 0, ctx->stream>>>(a);
+    else paged_split_kernel<D, 2><<<grid, kSplitThreads, 0, ctx->stream>>>(a);
+    LOGOS_LAUNCH_CHECK(ctx, "paged_split_kernel");
+    return LOGOS_OK;
+}
+
+}  // namespace
+
+size_t paged_attention_workspace_bytes(logos_ctx* ctx, const logos_paged_cache* c, const logos_paged_batch* b, int Hq) {
+    if (b->B == 0 || b->rows == 0 || b->max_q == 0) return kWorkspaceCounterBytes;
+    return plan_split(ctx, c, b, Hq / c->H).bytes;
+}
+
+int paged_attention(logos_ctx* ctx, int dtype, const void* Q, const logos_paged_cache* cache, const logos_paged_batch* batch,
+                    int Hq, const logos_attn_params* prm, void* O, const logos_row_strides* q_in, const logos_row_strides* o_out) {
+    if (int rc = paged_check(ctx, "paged_attention", cache, batch)) return rc;
+    if (dtype != LOGOS_BF16 && dtype != LOGOS_F16)
+        return fail(ctx, dtype_ok(dtype) ? LOGOS_ERR_UNSUPPORTED : LOGOS_ERR_INVALID_ARG, "paged_attention: Q and O are BF16 or FP16");
+    if (Hq <= 0 || Hq > 1024 || Hq % cache->H)
+        return fail(ctx, LOGOS_ERR_INVALID_ARG, "paged_attention: %d query heads over %d key/value heads (a multiple, at most 1024)", Hq, cache->H);
+    if (!(prm->scale > 0.0f) || !(prm->scale < INFINITY))
+        return fail(ctx, LOGOS_ERR_UNSUPPORTED, "paged_attention: scale must be positive and finite");
+    if (prm->ns_alpha > 0.0f && (prm->ns_eta != 0.0f || (prm->diffuse_mode != LOGOS_DIFFUSE_NONE && prm->ns_nu != 0.0f)))
+        return fail(ctx, LOGOS_ERR_UNSUPPORTED, "paged_attention: the Navier-Stokes terms are not offered over pages");
+    if (batch->B == 0 || batch->rows == 0 || batch->max_q == 0) return LOGOS_OK;
+    if (!Q || !O) return fail(ctx, LOGOS_ERR_INVALID_ARG, "paged_attention: null pointer");
+    if (!aligned16(Q) || !aligned16(O)) return fail(ctx, LOGOS_ERR_ALIGNMENT, "paged_attention: tensors must be 16-byte aligned");
+    const logos_row_strides packed{(int64_t)Hq * cache->DH, cache->DH};
+    const logos_row_strides q = q_in ? *q_in : packed, o = o_out ? *o_out : packed;
+    if (!rows_aligned(q, 2) || !rows_aligned(o, 2))
+        return fail(ctx, LOGOS_ERR_ALIGNMENT, "paged_attention: negative strides, or rows that are not 16-byte aligned");
+    if (!rows_apart(o, batch->rows, Hq, cache->DH))
+        return fail(ctx, LOGOS_ERR_INVALID_ARG, "paged_attention: the rows of the output overlap");
+    const int G = Hq / cache->H;
+    const SplitPlan plan = plan_split(ctx, cache, batch, G);
+    if ((int64_t)plan.splits * cache->H * plan.tiles > 0x7fffffffLL)
+        return fail(ctx, LOGOS_ERR_UNSUPPORTED, "paged_attention: the batch needs more than 2^31 CTAs");
+    if (!ctx->workspace || ctx->workspace_bytes < plan.bytes)
+        return fail(ctx, LOGOS_ERR_WORKSPACE, "paged_attention: needs %zu bytes of workspace, the context has %zu", plan.bytes,
+                    ctx->workspace ? ctx->workspace_bytes : 0);
+    SplitArgs a;
+    a.p = paged_args(ctx, cache, batch);
+    a.q = Q; a.o = O;
+    a.q_row = q.row; a.q_head = q.head; a.o_row = o.row; a.o_head = o.head;
+    a.c = prm->scale * 1.4426950408889634f;
+    a.G = G; a.is_f16 = dtype == LOGOS_F16;
+    a.causal = prm->causal != 0; a.window = prm->window; a.stride = prm->stride;
+    a.chunk = plan.chunk; a.splits = plan.splits; a.tiles = plan.tiles;
+    a.counters = static_cast<int*>(ctx->workspace);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(ctx->workspace) + kWorkspaceCounterBytes);
+    return cache->DH == 64 ? launch_split<64>(ctx, a, plan.rows) : launch_split<128>(ctx, a, plan.rows);
+}
+
+}  // namespace logos

@@ -234,6 +234,128 @@ class Engine:
                                                      S * DH))
         return scales
 
+    # ---- norm and rotation of queries and keys -----------------------------------
+    def _rows3(self, what, *tensors):
+        """Strides of [rows, H, DH] views (None stays None); the last dimension contiguous, one dtype, this device."""
+        first = next((t for t in tensors if t is not None), None)
+        if first is None:
+            raise ValueError(f"{what}: no tensor")
+        out = []
+        for t in tensors:
+            if t is None:
+                out.append(None)
+                continue
+            if t.dim() != 3 or (t.stride(2) != 1 and t.numel()):
+                raise ValueError(f"{what}: [rows, heads, DH] with contiguous channels, got {tuple(t.shape)} with strides {t.stride()}")
+            if t.dtype != first.dtype or t.shape[0] != first.shape[0] or t.shape[2] != first.shape[2]:
+                raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)} beside {first.dtype} {tuple(first.shape)}")
+            self._on_device(what, t)
+            out.append(C.byref(L.RowStrides(t.stride(0), t.stride(1))))
+        if first.dtype not in _DT:
+            raise ValueError(f"{what}: dtype {first.dtype}")
+        return out
+
+    def _on_device(self, what, *tensors):
+        for t in tensors:
+            if t is not None and (not t.is_cuda or t.device.index != self.device):
+                raise ValueError(f"{what}: a tensor on {t.device}, the engine is on cuda:{self.device}")
+
+    def _rope_args(self, what, Q, K, wq, wk, positions, rope):
+        rows, DH = (Q if Q is not None else K).shape[0::2]
+        for w in (wq, wk):
+            if w is not None and (w.dtype != torch.float32 or w.shape != (DH,) or not w.is_contiguous()):
+                raise ValueError(f"{what}: a weight is fp32 [{DH}], got {w.dtype} {tuple(w.shape)}")
+        if positions.dtype != torch.int32 or positions.shape != (rows,) or not positions.is_contiguous():
+            raise ValueError(f"{what}: positions are int32 [{rows}], got {positions.dtype} {tuple(positions.shape)}")
+        self._on_device(what, wq, wk, positions)
+        return rows, DH
+
+    def qk_norm_rope(self, Q, K, q_weight, k_weight, positions, rope, eps=1e-6, out_q=None, out_k=None):
+        """Every head of Q [rows, Hq, DH] and K [rows, Hk, DH] (views with any row and head strides; either may be None)
+        normalised by its RMS, weighted and rotated by its token's position, one kernel; a weight of None leaves that
+        norm out.  out_q / out_k: outputs (the inputs themselves for in place); None allocates packed ones."""
+        si = self._rows3("qk_norm_rope", Q, K)
+        rows, DH = self._rope_args("qk_norm_rope", Q, K, q_weight, k_weight, positions, rope)
+        out_q = torch.empty(Q.shape, dtype=Q.dtype, device=Q.device) if Q is not None and out_q is None else out_q
+        out_k = torch.empty(K.shape, dtype=K.dtype, device=K.device) if K is not None and out_k is None else out_k
+        so = self._rows3("qk_norm_rope", out_q, out_k)
+        for x, y in ((Q, out_q), (K, out_k)):
+            if (x is None) != (y is None) or (x is not None and (x.shape != y.shape or x.dtype != y.dtype)):
+                raise ValueError("qk_norm_rope: an output does not match its input")
+        self._check(self.lib.logos_qk_norm_rope(
+            self.h, _DT[(Q if Q is not None else K).dtype], _ptr(Q), _ptr(K), _ptr(q_weight), _ptr(k_weight), _ptr(positions),
+            C.byref(rope.desc), float(eps), _ptr(out_q), _ptr(out_k), rows, Q.shape[1] if Q is not None else 0,
+            K.shape[1] if K is not None else 0, DH, si[0], si[1], so[0], so[1]))
+        return out_q, out_k
+
+    def qk_norm_rope_bwd(self, Q, K, dQ_out, dK_out, q_weight, k_weight, positions, rope, eps=1e-6):
+        """Gradients (dQ, dK, dq_weight, dk_weight) of qk_norm_rope for the gradients of its outputs; dQ and dK packed in
+        the inputs' type, the weights' in fp32 (None where the weight, or the tensor, is None)."""
+        s = self._rows3("qk_norm_rope_bwd", Q, K, dQ_out, dK_out)
+        rows, DH = self._rope_args("qk_norm_rope_bwd", Q, K, q_weight, k_weight, positions, rope)
+        dx = []
+        for x, g, w in ((Q, dQ_out, q_weight), (K, dK_out, k_weight)):
+            if (x is None) != (g is None) or (x is not None and x.shape != g.shape) or (x is None and w is not None):
+                raise ValueError("qk_norm_rope_bwd: a gradient does not match its tensor")
+            dx.append(torch.empty(x.shape, dtype=x.dtype, device=x.device) if x is not None else None)
+        dwq, dwk = (torch.empty_like(w) if w is not None else None for w in (q_weight, k_weight))
+        args = (self.h, _DT[(Q if Q is not None else K).dtype], _ptr(Q), _ptr(K), _ptr(dQ_out), _ptr(dK_out), _ptr(q_weight),
+                _ptr(k_weight), _ptr(positions), C.byref(rope.desc), float(eps), _ptr(dx[0]), _ptr(dx[1]), _ptr(dwq), _ptr(dwk),
+                rows, Q.shape[1] if Q is not None else 0, K.shape[1] if K is not None else 0, DH, s[0], s[1], s[2], s[3],
+                None, None)
+        self._with_workspace(lambda: self.lib.logos_qk_norm_rope_bwd(*args),
+                             lambda: self.lib.logos_qk_norm_rope_bwd_workspace_bytes(DH))
+        return dx[0], dx[1], dwq, dwk
+
+    def _with_workspace(self, call, need):
+        """A call that reports a small workspace gets it reserved and runs again: no size query in the hot path."""
+        rc = call()
+        if rc == L.ERR_WORKSPACE:
+            self.reserve(need())
+            rc = call()
+        self._check(rc)
+
+    # ---- paged INT8 KV ---------------------------------------------------------
+    def paged_append(self, K, V, cache, batch):
+        """The batch's new K and V rows ([rows, H, DH], any row and head strides) quantised into their pages, a scale
+        per row.  rows may exceed the batch's last row: those are not read."""
+        s = self._rows3("paged_append", K, V)
+        self._paged_args("paged_append", K, V, cache, batch)
+        self._check(self.lib.logos_paged_append(self.h, _DT[K.dtype], _ptr(K), _ptr(V), s[0], s[1], C.byref(cache.desc),
+                                                C.byref(batch.desc)))
+
+    def paged_read(self, cache, batch, out_k, out_v):
+        """The values the cache holds for the batch's rows -> out_k, out_v ([rows, H, DH], fp32 or 16-bit, any row and
+        head strides); rows behind the last sequence stay as they are."""
+        s = self._rows3("paged_read", out_k, out_v)
+        self._paged_args("paged_read", out_k, out_v, cache, batch)
+        self._check(self.lib.logos_paged_read(self.h, _DT[out_k.dtype], C.byref(cache.desc), C.byref(batch.desc), _ptr(out_k),
+                                              _ptr(out_v), s[0], s[1]))
+        return out_k, out_v
+
+    def _paged_args(self, what, K, V, cache, batch):
+        if K.shape != V.shape or K.shape[1:] != (cache.heads, cache.dh):
+            raise ValueError(f"{what}: K {tuple(K.shape)}, V {tuple(V.shape)} for a cache of {cache.heads} heads of {cache.dh}")
+        self._on_device(what, cache.k, batch.cu_q)
+        batch.desc.rows = K.shape[0]
+
+    def paged_attention(self, Q, cache, batch, params: L.Params, out=None):
+        """Attention of the batch's new tokens Q [rows, Hq, DH] (BF16 or FP16, any row and head strides) over the pages
+        -> [rows, Hq, DH].  Append their K and V first.  With `out`, rows behind the last sequence stay as they are;
+        without it they are undefined."""
+        if out is None:
+            out = torch.empty(Q.shape, dtype=Q.dtype, device=Q.device)
+        s = self._rows3("paged_attention", Q, out)
+        if out.shape != Q.shape or Q.shape[2] != cache.dh:
+            raise ValueError(f"paged_attention: Q {tuple(Q.shape)}, out {tuple(out.shape)}, heads of {cache.dh} in the cache")
+        self._on_device("paged_attention", cache.k, batch.cu_q)
+        batch.desc.rows, Hq = Q.shape[0], Q.shape[1]
+        self._with_workspace(
+            lambda: self.lib.logos_paged_attention(self.h, _DT[Q.dtype], _ptr(Q), C.byref(cache.desc), C.byref(batch.desc), Hq,
+                                                   C.byref(params), _ptr(out), s[0], s[1]),
+            lambda: self.lib.logos_paged_attention_workspace_bytes(self.h, C.byref(cache.desc), C.byref(batch.desc), Hq))
+        return out
+
     # ---- Nikhilam INT8 KV ----------------------------------------------------
     def prefill(self, Q, K, V, params: L.Params, k_cache, v_cache, k_scale, v_scale, out_dtype=None, out=None):
         """One layer's prefill in one call: the raw K, V ([B,H,S,DH]) quantised into rows [0, S) of the

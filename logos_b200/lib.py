@@ -15,11 +15,37 @@ LIB_PATH = os.path.join(PKG, "liblogos_attn.so")
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_CUDA, ERR_NO_DEVICE, ERR_ALIGNMENT = range(7)
 ERR_SCRATCH_LIMIT = 7
 ERR_KERNEL_TIMEOUT = 8
+ERR_BAD_BATCH = 9
 F32, BF16, F16 = 0, 1, 2
 DIFFUSE_NONE, DIFFUSE_CAUSAL, DIFFUSE_CENTRAL = 0, 1, 2
 class Strides(C.Structure):
     """logos_strides: elements between two sequences, two heads, two rows."""
     _fields_ = [("batch", C.c_int64), ("head", C.c_int64), ("row", C.c_int64)]
+
+
+class RowStrides(C.Structure):
+    """logos_row_strides: elements between two rows (tokens) and two heads."""
+    _fields_ = [("row", C.c_int64), ("head", C.c_int64)]
+
+
+ROPE_MAX_PAIRS = 64
+
+
+class Rope(C.Structure):
+    """logos_rope."""
+    _fields_ = [("dims", C.c_int), ("interleaved", C.c_int), ("inv_freq", C.c_double * ROPE_MAX_PAIRS)]
+
+
+class PagedCache(C.Structure):
+    """logos_paged_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_int), ("page_size", C.c_int), ("H", C.c_int), ("DH", C.c_int)]
+
+
+class PagedBatch(C.Structure):
+    """logos_paged_batch."""
+    _fields_ = [("cu_q", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p), ("B", C.c_int),
+                ("max_pages", C.c_int), ("rows", C.c_int), ("max_q", C.c_int), ("max_kv", C.c_int)]
 
 
 MHA_ATTEND_DEQUANTIZED = 1
@@ -76,6 +102,15 @@ SIGNATURES = {
     "logos_decode_int8_gather": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _PP, _vp]),
     "logos_decode_step_int8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _PP, _vp]),
     "logos_decode_step_int8_to": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _PP, _i, _vp]),
+    "logos_qk_norm_rope": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, C.POINTER(Rope), _f, _vp, _vp, _i, _i, _i, _i, _vp, _vp,
+                                _vp, _vp]),
+    "logos_qk_norm_rope_bwd_workspace_bytes": (_sz, [_i]),
+    "logos_qk_norm_rope_bwd": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.POINTER(Rope), _f, _vp, _vp, _vp, _vp, _i,
+                                    _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "logos_paged_append": (_i, [_vp, _i, _vp, _vp, _vp, _vp, C.POINTER(PagedCache), C.POINTER(PagedBatch)]),
+    "logos_paged_read": (_i, [_vp, _i, C.POINTER(PagedCache), C.POINTER(PagedBatch), _vp, _vp, _vp, _vp]),
+    "logos_paged_attention_workspace_bytes": (_sz, [_vp, C.POINTER(PagedCache), C.POINTER(PagedBatch), _i]),
+    "logos_paged_attention": (_i, [_vp, _i, _vp, C.POINTER(PagedCache), C.POINTER(PagedBatch), _i, _PP, _vp, _vp, _vp]),
     "logos_layer_norm": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, C.c_float]),
     "logos_decode_step_int8_gather": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i,
                                           _PP, _vp]),
