@@ -52,4 +52,33 @@ __host__ __device__ __forceinline__ size_t paged_row(const PagedArgs& a, int pag
     return ((size_t)page * a.H + h) << a.page_shift;
 }
 
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+    return r;
+}
+// two biased bytes (b + 128) under the exponent of 1024, minus 1152
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t biased, uint32_t sel) {
+    const uint32_t w = prmt(biased, 0x64646464u, sel), bias = 0x64806480u;
+    __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// A query row in FP16 by a power of two: `top` = max|q| of the row.  The factor puts it at 2^13 ... 2^14, so a BF16
+// row keeps every bit of values down to 2^-27 of its largest; rows of zeros, infinities or NaN keep factor 1.
+__device__ __forceinline__ void row_power(float top, float& mul, float& inv) {
+    const int be = (int)(__float_as_uint(top) >> 23);
+    const int up = (be == 0 || be >= 255) ? 127 : min(max(267 - be, 1), 253);   // biased exponent of the factor
+    mul = __uint_as_float((uint32_t)up << 23);
+    inv = __uint_as_float((uint32_t)(254 - up) << 23);
+}
+
+// paged_chunk.cu: the sequences with more than min_rows query rows per key/value head
+size_t paged_chunk_workspace_bytes(const logos_ctx* ctx, int DH);
+int paged_chunk(logos_ctx* ctx, const PagedArgs& p, int DH, const void* Q, void* O, const logos_row_strides& q,
+                const logos_row_strides& o, int G, bool f16, const logos_attn_params* prm, int min_rows);
+
+constexpr float kMoveMax = 8.0f;          // log2 units by which a row may outgrow its reference maximum (weights stay below 2^8 in FP16)
+constexpr float kLeastScale = 1e-30f;     // a value scale below this (a row nobody wrote) counts as this: its log2 stays finite
+
 }  // namespace logos

@@ -29,7 +29,7 @@ namespace {
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = 32 * kSplitWarps;
 constexpr int kSpan = 2048;                      // keys whose pages a warp's lanes hold, one 16-key block each
-constexpr float kMoveMax = 8.0f;                 // log2 units by which a row may outgrow its reference maximum
+constexpr int kFewRows = 32;                     // query rows per head up to which a sequence is this kernel's
 constexpr int kSplitCounters = (int)(kWorkspaceCounterBytes / sizeof(int));
 
 struct SplitArgs {
@@ -39,22 +39,12 @@ struct SplitArgs {
     long long q_row, q_head, o_row, o_head;
     float c;                                     // scale * log2(e)
     int G, is_f16, causal, window, stride;
+    int max_rows;                                // sequences with more query rows per head belong to paged_chunk_kernel
     int chunk, splits, tiles;                    // keys per chunk; most chunks and row tiles of a (sequence, head)
     float* part;                                 // [(sequence, head, tile)][splits][rows][DH + 2]
     int* counters;
 };
 
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-    uint32_t r;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
-    return r;
-}
-// two biased bytes (b + 128) under the exponent of 1024, minus 1152
-__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t biased, uint32_t sel) {
-    const uint32_t w = prmt(biased, 0x64646464u, sel), bias = 0x64806480u;
-    __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&bias));
-    return *reinterpret_cast<uint32_t*>(&h);
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -96,7 +86,7 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
         return;
     }
     const int r0 = tile * ROWS, n_rows = min(ROWS, s.n * a.G - r0);
-    if (n_rows <= 0) return;
+    if (n_rows <= 0 || (long long)s.n * a.G > a.max_rows) return;
     const int first = s.kv - s.n + r0 / a.G, last = s.kv - s.n + (r0 + n_rows - 1) / a.G;   // positions of the tile's rows
     const bool shun = shunyam_active(a.window, s.kv);
     const bool pure = shun && a.stride <= 0;     // a window without landmarks bounds the keys on both sides
@@ -197,10 +187,9 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int be = (int)(__float_as_uint(top) >> 23);
-        const int up = (be == 0 || be == 255) ? 127 : min(max(267 - be, 1), 253);   // biased exponent of the power of two
-        const float mul = __uint_as_float((uint32_t)up << 23);
-        alpha[n] = a.c * __uint_as_float((uint32_t)(254 - up) << 23);
+        float mul, unmul;
+        row_power(top, mul, unmul);
+        alpha[n] = a.c * unmul;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const __half2 lo = __floats2half2_rn(f[4 * ks] * mul, f[4 * ks + 1] * mul), hi = __floats2half2_rn(f[4 * ks + 2] * mul, f[4 * ks + 3] * mul);
@@ -237,7 +226,7 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mma_f16(sc[u], qa[4 * i + e], bytes_to_half2(w[e], 0x4140), bytes_to_half2(w[e], 0x4342));
             }
-            const float v0 = fmaxf(vsr[u].x, 1e-30f), v1 = fmaxf(vsr[u].y, 1e-30f);
+            const float v0 = fmaxf(vsr[u].x, kLeastScale), v1 = fmaxf(vsr[u].y, kLeastScale);
             const float b0 = __log2f(v0), b1 = __log2f(v1);
             inv[u] = make_float2(__fdividef(1.0f, v0), __fdividef(1.0f, v1));
 #pragma unroll
@@ -399,10 +388,12 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
 }
 
 // how a batch is cut: row tiles of 8 or 16, chunks of keys
-struct SplitPlan { int rows, tiles, chunk, splits; size_t bytes; };
+struct SplitPlan { int rows, tiles, chunk, splits; size_t bytes; bool chunks; };
 SplitPlan plan_split(const logos_ctx* ctx, const logos_paged_cache* c, const logos_paged_batch* b, int G) {
     SplitPlan p;
-    const int64_t most = (int64_t)b->max_q * G;              // query rows of a (sequence, head)
+    int64_t most = (int64_t)b->max_q * G;                    // query rows of a (sequence, head)
+    p.chunks = most > kFewRows;                              // some may be paged_chunk_kernel's
+    if (p.chunks) most = kFewRows;
     p.rows = most <= 8 ? 8 : 16;
     p.tiles = (int)((most + p.rows - 1) / p.rows);
     const int64_t units = (int64_t)b->B * c->H * p.tiles;
@@ -415,6 +406,10 @@ SplitPlan plan_split(const logos_ctx* ctx, const logos_paged_cache* c, const log
     p.chunk = chunk < 128 ? 128 : (int)chunk;
     p.splits = (b->max_kv + p.chunk - 1) / p.chunk;
     p.bytes = kWorkspaceCounterBytes + (size_t)units * p.splits * p.rows * (c->DH + 2) * sizeof(float);
+    if (p.chunks) {                                          // the two kernels run one after the other
+        const size_t other = paged_chunk_workspace_bytes(ctx, c->DH);
+        if (other > p.bytes) p.bytes = other;
+    }
     return p;
 }
 
@@ -468,10 +463,13 @@ int paged_attention(logos_ctx* ctx, int dtype, const void* Q, const logos_paged_
     a.c = prm->scale * 1.4426950408889634f;
     a.G = G; a.is_f16 = dtype == LOGOS_F16;
     a.causal = prm->causal != 0; a.window = prm->window; a.stride = prm->stride;
+    a.max_rows = kFewRows;
     a.chunk = plan.chunk; a.splits = plan.splits; a.tiles = plan.tiles;
     a.counters = static_cast<int*>(ctx->workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(ctx->workspace) + kWorkspaceCounterBytes);
-    return cache->DH == 64 ? launch_split<64>(ctx, a, plan.rows) : launch_split<128>(ctx, a, plan.rows);
+    if (int rc = cache->DH == 64 ? launch_split<64>(ctx, a, plan.rows) : launch_split<128>(ctx, a, plan.rows)) return rc;
+    if (!plan.chunks) return LOGOS_OK;
+    return paged_chunk(ctx, a.p, cache->DH, Q, O, q, o, G, a.is_f16 != 0, prm, kFewRows);
 }
 
 }  // namespace logos
