@@ -63,6 +63,12 @@ __device__ __forceinline__ uint32_t bytes_to_half2(uint32_t biased, uint32_t sel
     __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&bias));
     return *reinterpret_cast<uint32_t*>(&h);
 }
+// two raw bytes u under 0x43: BF16 128 + (u & 127), minus 128 or, for a negative one, 256
+__device__ __forceinline__ uint32_t bytes_to_bf162(uint32_t bytes, uint32_t sel) {
+    const uint32_t w = prmt(bytes, 0x43434343u, sel), p = w & 0xff7fff7fu, c = w & 0xff80ff80u;
+    __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&p), *reinterpret_cast<const __nv_bfloat162*>(&c));
+    return *reinterpret_cast<uint32_t*>(&r);
+}
 
 // A query row in FP16 by a power of two: `top` = max|q| of the row.  The factor puts it at 2^13 ... 2^14, so a BF16
 // row keeps every bit of values down to 2^-27 of its largest; rows of zeros, infinities or NaN keep factor 1.
@@ -78,7 +84,7 @@ size_t paged_chunk_workspace_bytes(const logos_ctx* ctx, int DH);
 int paged_chunk(logos_ctx* ctx, const PagedArgs& p, int DH, const void* Q, void* O, const logos_row_strides& q,
                 const logos_row_strides& o, int G, bool f16, const logos_attn_params* prm, int min_rows);
 
-constexpr float kMoveMax = 8.0f;          // log2 units by which a row may outgrow its reference maximum (weights stay below 2^8 in FP16)
+constexpr float kMoveMax = 15.0f;         // log2 units by which a row may outgrow its reference maximum (weights up to 2^15: FP16 ends at 2^16)
 constexpr float kLeastScale = 1e-30f;     // a value scale below this (a row nobody wrote) counts as this: its log2 stays finite
 
 }  // namespace logos

@@ -116,36 +116,43 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
     uint4 kr[KG][D / 64];
     uint32_t vr[KB / 4][VW];
     float2 ksr[KG], vsr[KG];
+    // A page that is not there is read as page 0 and masked later: no load waits for a test.
     auto load_k = [&](int it) {
+        if (it >= n_iter) return;
 #pragma unroll
-        for (int u = 0; u < KG; ++u) {
-            const int page = __shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + (u >> 1)) & 31);
-            const int key = s0 + (it * kSplitWarps + warp) * KB + 8 * u;
-            const bool in = page >= 0 && it < n_iter;
-            const size_t row = paged_row(a.p, in ? page : 0, h) + (key & ((1 << a.p.page_shift) - 1));
+        for (int u2 = 0; u2 < KG / 2; ++u2) {
+            const int page = max(__shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + u2) & 31), 0);
+            const int key = s0 + (it * kSplitWarps + warp) * KB + 16 * u2;
+            const size_t row = paged_row(a.p, page, h) + (key & ((1 << a.p.page_shift) - 1));
+            const uint4* at = reinterpret_cast<const uint4*>(a.p.k + (row + g) * D) + t;
+            const float2* sk = reinterpret_cast<const float2*>(a.p.ks + row) + t;
+            const float2* sv = reinterpret_cast<const float2*>(a.p.vs + row) + t;
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i)
-                kr[u][i] = in ? __ldg(reinterpret_cast<const uint4*>(a.p.k + (row + g) * D + 64 * i + 16 * t)) : make_uint4(0, 0, 0, 0);
-            ksr[u] = in ? __ldg(reinterpret_cast<const float2*>(a.p.ks + row + 2 * t)) : make_float2(0.0f, 0.0f);
-            vsr[u] = in ? __ldg(reinterpret_cast<const float2*>(a.p.vs + row + 2 * t)) : make_float2(1.0f, 1.0f);
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) kr[2 * u2 + e][i] = __ldg(at + 8 * e * (D / 16) + 4 * i);
+                ksr[2 * u2 + e] = __ldg(sk + 4 * e);
+                vsr[2 * u2 + e] = __ldg(sv + 4 * e);
+            }
         }
     };
     auto load_v = [&](int it) {
+        if (it >= n_iter) return;
 #pragma unroll
-        for (int u = 0; u < KG; ++u) {
-            const int page = __shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + (u >> 1)) & 31);
-            const int key = s0 + (it * kSplitWarps + warp) * KB + 8 * u;
-            const bool in = page >= 0 && it < n_iter;
-            const size_t row = paged_row(a.p, in ? page : 0, h) + (key & ((1 << a.p.page_shift) - 1)) + 2 * t;
+        for (int u2 = 0; u2 < KG / 2; ++u2) {
+            const int page = max(__shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + u2) & 31), 0);
+            const int key = s0 + (it * kSplitWarps + warp) * KB + 16 * u2;
+            const size_t row = paged_row(a.p, page, h) + (key & ((1 << a.p.page_shift) - 1)) + 2 * t;
+            const int8_t* at = a.p.v + row * D + g * (D / 8);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int8_t* at = a.p.v + (row + i) * D + g * (D / 8);
+            for (int i = 0; i < 4; ++i) {                // keys 2t, 2t + 1, 2t + 8, 2t + 9
+                const int8_t* w = at + (8 * (i >> 1) + (i & 1)) * D;
                 if (D == 64) {
-                    const uint2 w = in ? __ldg(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
-                    vr[2 * u + i][0] = w.x; vr[2 * u + i][1] = w.y;
+                    const uint2 x = __ldg(reinterpret_cast<const uint2*>(w));
+                    vr[4 * u2 + i][0] = x.x; vr[4 * u2 + i][1] = x.y;
                 } else {
-                    const uint4 w = in ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0, 0, 0, 0);
-                    vr[2 * u + i][0] = w.x; vr[2 * u + i][1] = w.y; vr[2 * u + i][VW - 2] = w.z; vr[2 * u + i][VW - 1] = w.w;
+                    const uint4 x = __ldg(reinterpret_cast<const uint4*>(w));
+                    vr[4 * u2 + i][0] = x.x; vr[4 * u2 + i][1] = x.y; vr[4 * u2 + i][VW - 2] = x.z; vr[4 * u2 + i][VW - 1] = x.w;
                 }
             }
         }
@@ -259,7 +266,7 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
             for (int u = 1; u < KG; ++u) top = fmaxf(top, fmaxf(sc[u][2 * n], sc[u][2 * n + 1]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // the reference maximum moves only when a weight would pass 2^8 (well inside FP16), or at the first key
+            // the reference maximum moves only when a weight would pass 2^15 (FP16 ends at 2^16), or at the first key
             const bool move = top > m[n] + kMoveMax || (m[n] == -INFINITY && top > -INFINITY);
             f[n] = (move && m[n] > -INFINITY) ? exp2_fast(m[n] - top) : 1.0f;
             moved |= move && m[n] > -INFINITY;

@@ -10,14 +10,14 @@
 // per 256 rows and comes from L2 after the first.  So the threads' chain per tile decides, and everything that is not
 // softmax is taken off the softmax threads.
 //
-// A CTA (512 threads, one per SM) holds two 128-row tiles of one (sequence, head) -- row r is token r / G, query head
+// A CTA (896 threads, one per SM) holds two 128-row tiles of one (sequence, head) -- row r is token r / G, query head
 // r % G of the group, so grouped heads share every K and V tile -- and walks over key tiles of 128.  Roles:
-//   warps 0-3 / 4-7   softmax of tile 0 / 1, one thread per row (TMEM lane), the row's 128 scores in registers
-//   warps 8,9 / 10,11 K / V: pages -> registers one tile ahead -> FP16 -> 128B-swizzled tiles in shared memory
-//   warps 12,13       MMA issuers, one per tile: S = Q K^T from shared memory, O += P V with P read from TMEM
-//   warp 14           the schedule
+//   warps 0-7 / 8-15  softmax of tile 0 / 1, 16 rows a warp
+//   warps 16-19 / 20-23 K / V: pages -> shared memory, asynchronously -> 16 bits -> 128B-swizzled tiles in shared memory
+//   warps 24,25       MMA issuers, one per tile: S = Q K^T from shared memory, O += P V with P read from TMEM
+//   warp 26           the schedule
 // TMEM (512 columns), DH 64: S 2 x 128, O 2 x 64, P 2 x 64, so the next scores are computed under this tile's
-// exponentials.  DH 128: S 2 x 128, O 2 x 128; P lies on the first half of its own S, the next scores follow this
+// exponentials.  DH 128: S 2 x 128, O 2 x 128; P lies on the second half of its own S, the next scores follow this
 // tile's PV in the pipe and the other tile's exponentials cover both.
 //
 // Schedule.  The key tiles of all (sequence, head, 256 rows) items form one line, cut into equal shares, one per CTA:
@@ -32,21 +32,77 @@ namespace {
 
 using namespace tc;
 
-constexpr int kChunkThreads = 512;
+constexpr int kChunkThreads = 896;
 constexpr int kChunkRows = 256;              // query rows of an item
 constexpr int kBN = 128;                     // keys of a tile
-constexpr int kConvWarp = 8, kMmaWarp = 12, kPlanWarp = 14;
-constexpr int kRegsSoftmax = 184, kRegsConvert = 104, kRegsRest = 40;
-static_assert(256 * kRegsSoftmax + 128 * kRegsConvert + 128 * kRegsRest <= 65536 && 65536 / kChunkThreads == 128, "registers");
+constexpr int kConvWarp = 16, kMmaWarp = 24, kPlanWarp = 26;
+constexpr int kRegsSoftmax = 88, kRegsConvert = 48, kRegsRest = 56;      // the launch gives every thread 72
+static_assert(512 * kRegsSoftmax + 256 * kRegsConvert + 128 * kRegsRest <= kChunkThreads * 72 && kChunkThreads * 72 <= 65536, "registers");
 constexpr int kScaleStages = 4, kSegStages = 4;
-constexpr int kSegReaders = kPlanWarp;       // warps 0 ... 13 read every segment
+constexpr int kSegReaders = kPlanWarp;       // warps 0 ... 25 read every segment
+constexpr float kLeastFactor = 1e-37f;
+constexpr float kNoReference = -1e30f;       // reference of a row that has seen no key: any visible key lies above it
 constexpr int kJoinRows = 32;                // rows a CTA of the join takes
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// One poll of a barrier, asleep for up to 20 us; a waiting warp that polls by itself takes issue slots from the working ones.
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000) : "memory");
     return ok != 0;
+}
+// Bounded wait of a whole warp with one verdict: false when the CTA is aborting (this wait or another one ran out).
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    for (uint32_t it = 0; it < (1u << 16); ++it) {
+        if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+        if ((it & 15u) == 15u && __any_sync(0xffffffffu, *abort_flag != 0)) return false;
+    }
+    // as mbar_wait records it: the barrier's address and the thread
+    atomicCAS(const_cast<int*>(abort_flag), 0, (int)((bar & 0xffffu) | (threadIdx.x << 16)) | 0x40000000);
+    return false;
+}
+
+// TMEM accesses of 16 lanes x 256 (128) bits: thread t of the warp holds lanes t / 4 and t / 4 + 8.
+// 256 bits: registers 4 b ... 4 b + 3 are columns 8 b + 2 (t % 4), + 1 of the first lane, then of the second; 128 bits:
+// registers 2 w, 2 w + 1 are column 4 w + t % 4 of the two lanes.
+__device__ __forceinline__ void tc_ld_16x256_x4(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tc_st_16x256_x4(uint32_t taddr, const float* v) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tc_ld_16x128_x4(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.16x128b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_st_16x128_x4(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+                 : "memory");
+}
+constexpr int kBW = 32;                       // keys a softmax warp works on at once
+__device__ __forceinline__ void ld_scores(uint32_t taddr, float (&x)[kBW / 2]) {
+#pragma unroll
+    for (int i = 0; i < kBW / 32; ++i) tc_ld_16x256_x4(taddr + 32 * i, x + 16 * i);
 }
 
 template <int D> struct Shape {
@@ -56,11 +112,13 @@ template <int D> struct Shape {
     static constexpr int kOffQ = 0, kOffK = kOffQ + 2 * kTile, kOffV = kOffK + kStages * kTile;
     static constexpr int kOffScale = kOffV + kStages * kTile; // kScaleStages x {a, b, 1/vs: 128 floats each, 4 words of landmarks}
     static constexpr int kScaleBytes = 3 * kBN * 4 + 16;
-    static constexpr int kOffSeg = kOffScale + kScaleStages * kScaleBytes;
+    static constexpr int kDepth = D == 64 ? 4 : 3;            // pieces of 1 KiB a converting warp has in flight
+    static constexpr int kOffRaw = kOffScale + kScaleStages * kScaleBytes;
+    static constexpr int kOffSeg = kOffRaw + 8 * kDepth * 1024;
     static constexpr int kOffBar = kOffSeg + kSegStages * 64;
     static constexpr int kNumBars = 4 * kStages + 2 * kScaleStages + 2 * kSegStages + 5 * 2 + 1;
     static constexpr int kOffScan = kOffBar + kNumBars * 8;
-    static constexpr int kSmem = kOffScan + 128 + 1024;       // + alignment slack
+    static constexpr int kSmem = kOffScan + 8 * (kChunkThreads / 32) + 1024;       // + alignment slack
     static constexpr int kColO = 256, kColP = 384;
 };
 static_assert(Shape<128>::kSmem <= 232448 && Shape<64>::kSmem <= 232448, "shared memory");
@@ -133,12 +191,12 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int i = 0; i < ST; ++i) { mbar_init(bar(KFULL + i), 64); mbar_init(bar(KEMPTY + i), 2); mbar_init(bar(VFULL + i), 64); mbar_init(bar(VEMPTY + i), 2); }
-        for (int i = 0; i < kScaleStages; ++i) { mbar_init(bar(SCFULL + i), 64); mbar_init(bar(SCEMPTY + i), 256); }
+        for (int i = 0; i < ST; ++i) { mbar_init(bar(KFULL + i), 4); mbar_init(bar(KEMPTY + i), 2); mbar_init(bar(VFULL + i), 4); mbar_init(bar(VEMPTY + i), 2); }
+        for (int i = 0; i < kScaleStages; ++i) { mbar_init(bar(SCFULL + i), 4); mbar_init(bar(SCEMPTY + i), 16); }
         for (int i = 0; i < kSegStages; ++i) { mbar_init(bar(SEGFULL + i), 1); mbar_init(bar(SEGEMPTY + i), kSegReaders); }
         for (int g = 0; g < 2; ++g) {
-            mbar_init(bar(SFULL + g), 1); mbar_init(bar(SEMPTY + g), 128); mbar_init(bar(PFULL + g), 128);
-            mbar_init(bar(PVDONE + g), 1); mbar_init(bar(QREADY + g), 128);
+            mbar_init(bar(SFULL + g), 1); mbar_init(bar(SEMPTY + g), 8); mbar_init(bar(PFULL + g), 8);
+            mbar_init(bar(PVDONE + g), 1); mbar_init(bar(QREADY + g), 8);
         }
         mbar_init(bar(DRAIN), 2);
         abort_word = 0;
@@ -246,15 +304,16 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
             uint32_t elected;
             asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(elected));
             const bool leader = elected != 0;
-            auto wait_w = [&](uint32_t bb, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bb, parity, abort_flag)) != 0; };
-            constexpr uint32_t idesc_qk = instr_desc(0, 0, 0, kBN), idesc_pv = instr_desc(0, 0, 1 /* V is MN-major */, D);
+            auto wait_w = [&](uint32_t bb, uint32_t parity) { return wait_warp(bb, parity, abort_flag); };
+            const uint32_t idesc_qk = instr_desc(a.is_f16 ? 0 : 1, a.is_f16 ? 0 : 1, 0, kBN);
+            constexpr uint32_t idesc_pv = instr_desc(0, 0, 1 /* V is MN-major */, D);
             const uint32_t desc_hi = (uint32_t)(smem_desc(0) >> 32);
             // K-major: the leading offset is not used; MN-major: 64 channels are one swizzle atom, the next 64 lie 16 KiB on
             auto lo_of = [](uint32_t addr, uint32_t lead) { return ((addr >> 4) & 0x3FFFu) | ((lead >> 4) << 16); };
             auto desc = [&](uint32_t lo) { return ((uint64_t)desc_hi << 32) | lo; };
             const uint32_t q_lo = lo_of(sbase + C::kOffQ + g * C::kTile, 16), k_lo0 = lo_of(sbase + C::kOffK, 16), v_lo0 = lo_of(sbase + C::kOffV, 16384);
             const uint32_t d_s = tmem + (uint32_t)g * 128u, d_o = tmem + C::kColO + (uint32_t)(g * D);
-            const uint32_t a_p = C::kOwnP ? tmem + C::kColP + (uint32_t)g * 64u : d_s;
+            const uint32_t a_p = C::kOwnP ? tmem + C::kColP + (uint32_t)g * 64u : d_s + 64u;
             int nk = 0, nv = 0, s_qk = 0, s_pv = 0, n_seg = 0;
             bool ok = true;
             for (; ok; ++n_seg) {
@@ -331,331 +390,411 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
             // nothing of this warp is in flight when the CTA gives its tensor memory back, aborted or not
             if (leader) tc_commit(bar(DRAIN));
             __syncwarp();
-            for (uint32_t it = 0; it < kSpinLimit && !mbar_try(bar(DRAIN), 0); ++it) {}
+            for (uint32_t it = 0; it < (1u << 16) && !mbar_try(bar(DRAIN), 0); ++it) {}
         }
     } else if (warp >= kConvWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
         if (work) {
-            // ================= K (warps 8, 9) and V (10, 11) to FP16 =================
-            constexpr int LR = D / 16, RI = 32 / LR, NI = 64 / RI;   // lanes of a row, rows of a load, loads of a tile's half
-            const bool is_v = warp >= kConvWarp + 2;
-            const int w64 = 64 * (warp & 1);                         // this warp's rows of the tile
+            // ================= K (warps 16-19) and V (20-23) to 16 bits =================
+            // A warp takes 32 rows of every tile as pieces of 1 KiB (16 or 8 keys), which never cross a page.  A piece's bytes wait
+            // in shared memory, each where the thread that fetched it will read it (no barrier), kDepth pieces in flight.
+            constexpr int LR = D / 16, RI = 32 / LR;                 // lanes of a row, rows of a load
+            constexpr int PR = 1024 / D, NP = PR / RI, PPT = 32 / PR;   // rows and loads of a piece, pieces of the warp's share of a tile
+            const bool is_v = warp >= kConvWarp + 4;
+            const int part = warp & 3, w32 = 32 * part;              // this warp's rows of the tile
             const int FULL = is_v ? VFULL : KFULL, EMPTY = is_v ? VEMPTY : KEMPTY;
             unsigned char* tiles = smem + (is_v ? C::kOffV : C::kOffK);
             const int8_t* src = is_v ? a.p.v : a.p.k;
-            const int c16 = lane % LR;                               // 16 channels of a row
+            auto wait_w = [&](uint32_t bb, uint32_t parity) { return wait_warp(bb, parity, abort_flag); };
+            auto arrive_w = [&](uint32_t bb) { __syncwarp(); if (lane == 0) mbar_arrive(bb); };
+            const int c16 = lane % LR, r16 = lane / LR;              // 16 channels, first row of a piece
+            unsigned char* raw = smem + C::kOffRaw + (warp - kConvWarp) * (C::kDepth * 1024) + lane * 16;
+            const uint32_t raw_addr = smem_u32(raw);
+            const int page_mask = (1 << a.p.page_shift) - 1;
+            const int ch = 2 * (c16 & 3);
+            const bool bf16 = !is_v && !a.is_f16;                    // K in the type of the queries, V in that of the weights
             int n_t = 0;
             bool ok = true;
             for (int n_seg = 0; ok; ++n_seg) {
                 const int sst = n_seg % kSegStages;
-                if (!__all_sync(0xffffffffu, mbar_wait(bar(SEGFULL + sst), (n_seg / kSegStages) & 1, abort_flag))) break;
-                const Segment sg = *reinterpret_cast<const Segment*>(smem + C::kOffSeg + sst * 64);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(SEGEMPTY + sst));
-                if (sg.n_iter == 0) break;
-                // Pages, eight tiles at a time and the next eight ahead: lane 4 i + j holds the page of keys 16 j ... of this
-                // warp's half of tile i.
-                auto pages_from = [&](int i) {
-                    const int key = sg.begin + (sg.i0 + i + (lane >> 2)) * kBN + w64 + 16 * (lane & 3);
-                    if (i + (lane >> 2) >= sg.n_iter || key >= sg.end) return -1;
-                    const int page = paged_page(a.p, sg.b, key);
-                    if (page < 0) report_batch(a.p.status, sg.b, true);
-                    return page;
+                if (!wait_w(bar(SEGFULL + sst), (n_seg / kSegStages) & 1)) break;
+                const Segment* seg = reinterpret_cast<const Segment*>(smem + C::kOffSeg + sst * 64);
+                const int sb = seg->b, sh = seg->h, n_iter = seg->n_iter, key_first = seg->begin + seg->i0 * kBN + w32, end = seg->end;
+                arrive_w(bar(SEGEMPTY + sst));
+                if (n_iter == 0) break;
+                // Table entries, 16 tiles at a time and the next 16 ahead: lane 2 i + j holds that of keys 16 j ... of this
+                // warp's quarter of tile i (0 where there is no key).
+                auto entries_from = [&](int i) {
+                    const int key = key_first + (i + (lane >> 1)) * kBN + 16 * (lane & 1);
+                    if (i + (lane >> 1) >= n_iter || key >= end) return 0;
+                    return a.p.table[(size_t)sb * a.p.max_pages + (key >> a.p.page_shift)];
                 };
-                int pg = pages_from(0), pg_next = pages_from(8);
-                uint4 buf[NI];
-                float2 ks = make_float2(0.0f, 0.0f), vs = make_float2(0.0f, 0.0f);
-                bool there = false;                                  // the two keys whose scales this thread holds
-                auto load_tile = [&](int i) {                        // tile i of the segment; nothing beyond its last
-                    if (i >= sg.n_iter) return;
-                    if ((i & 7) == 0 && i > 0) { pg = pg_next; pg_next = pages_from(i + 8); }
-                    const int key0 = sg.begin + (sg.i0 + i) * kBN + w64;
+                auto checked = [&](int page) {                       // -1: outside the cache
+                    if ((unsigned)page < (unsigned)a.p.pages) return page;
+                    report_batch(a.p.status, sb, true);
+                    return -1;
+                };
+                int pg = checked(entries_from(0)), pg_next = entries_from(16);
+                float ks = 0.0f, vs = 0.0f;                          // the scales of this thread's key of the tile
+                bool there = false;
+                int slot_in = 0, slot_out = 0;
+                // fetch piece n of the segment; with a tile's first piece also its scales.  A page that is not there is read as
+                // page 0: its keys weigh nothing, and no load waits for a test.
+                auto fetch = [&](int n) {
+                    if (n < PPT * n_iter) {
+                        const int i = n / PPT, blk = n % PPT;
+                        if (n % (16 * PPT) == 0 && n > 0) { pg = checked(pg_next); pg_next = entries_from(i + 16); }
+                        const int key = key_first + i * kBN + PR * blk;
+                        const int page = max(__shfl_sync(0xffffffffu, pg, 2 * (i & 15) + (PR * blk >> 4)), 0);
+                        const int8_t* at = src + (paged_row(a.p, page, sh) + (key & page_mask) + r16) * D + 16 * c16;
 #pragma unroll
-                    for (int u = 0; u < NI; ++u) {
-                        const int r = RI * u + lane / LR;
-                        const int page = __shfl_sync(0xffffffffu, pg, 4 * (i & 7) + (RI * u >> 4));
-                        const size_t row = paged_row(a.p, page < 0 ? 0 : page, sg.h) + ((key0 + r) & ((1 << a.p.page_shift) - 1));
-                        buf[u] = page >= 0 ? __ldg(reinterpret_cast<const uint4*>(src + row * D) + c16) : make_uint4(0, 0, 0, 0);
+                        for (int u = 0; u < NP; ++u) cp_async16(raw_addr + slot_in * 1024 + u * 512, at + u * RI * D);
+                        slot_in = slot_in + 1 == C::kDepth ? 0 : slot_in + 1;
                     }
-                    if (!is_v) {
-                        const int page = __shfl_sync(0xffffffffu, pg, 4 * (i & 7) + (lane >> 3));
-                        const int key = key0 + 2 * lane;
-                        there = page >= 0;
-                        const size_t row = paged_row(a.p, there ? page : 0, sg.h) + (key & ((1 << a.p.page_shift) - 1));
-                        if (there) {
-                            ks = __ldg(reinterpret_cast<const float2*>(a.p.ks + row));
-                            vs = __ldg(reinterpret_cast<const float2*>(a.p.vs + row));
-                        }
-                    }
+                    cp_async_commit();
                 };
-                load_tile(0);
-                for (int i = 0; ok && i < sg.n_iter; ++i, ++n_t) {
+                auto fetch_scales = [&](int i) {
+                    if (is_v || i >= n_iter) return;
+                    const int key = key_first + i * kBN + lane;
+                    const int page = __shfl_sync(0xffffffffu, (i & 15) == 0 && i > 0 ? pg_next : pg, 2 * (i & 15) + (lane >> 4));
+                    there = (unsigned)page < (unsigned)a.p.pages && key < end;
+                    const size_t row = paged_row(a.p, there ? page : 0, sh) + (key & page_mask);
+                    ks = __ldg(a.p.ks + row);
+                    vs = __ldg(a.p.vs + row);
+                };
+                fetch_scales(0);
+#pragma unroll 1
+                for (int n = 0; n < C::kDepth - 1; ++n) fetch(n);
+                for (int i = 0; ok && i < n_iter; ++i, ++n_t) {
                     if (!is_v) {
                         const int sc = n_t % kScaleStages;
-                        if (n_t >= kScaleStages && !__all_sync(0xffffffffu, mbar_wait(bar(SCEMPTY + sc), ((n_t / kScaleStages) - 1) & 1, abort_flag))) { ok = false; break; }
-                        float* sa = reinterpret_cast<float*>(smem + C::kOffScale + sc * C::kScaleBytes);
-                        const int key0 = sg.begin + (sg.i0 + i) * kBN + w64, j = w64 + 2 * lane;
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const bool in = there && key0 + 2 * lane + e < sg.end;      // a key that is not there weighs 2^-inf
-                            const float v = fmaxf(e ? vs.y : vs.x, kLeastScale);
-                            sa[j + e] = in ? a.c * (e ? ks.y : ks.x) : 0.0f;
-                            sa[kBN + j + e] = in ? __log2f(v) : -INFINITY;
-                            sa[2 * kBN + j + e] = in ? __fdividef(1.0f, v) : 0.0f;
+                        if (n_t >= kScaleStages && !wait_w(bar(SCEMPTY + sc), ((n_t / kScaleStages) - 1) & 1)) { ok = false; break; }
+                        float* sa = reinterpret_cast<float*>(smem + C::kOffScale + sc * C::kScaleBytes) + w32;
+                        const float v = fmaxf(vs, kLeastScale);
+                        // A key that is not there weighs 2^-inf.  The factor of a score is never 0, so that the -inf of a masked score
+                        // stays one.
+                        sa[lane] = there ? fmaxf(a.c * ks, kLeastFactor) : kLeastFactor;
+                        sa[kBN + lane] = there ? fminf(__log2f(v), 3e38f) : -INFINITY;   // finite: a masked score keeps its -inf beside an infinite scale
+                        sa[2 * kBN + lane] = there ? __fdividef(1.0f, v) : 0.0f;
+                        if (a.stride > 0) {                                               // landmark bits of the warp's keys
+                            const uint32_t m = __ballot_sync(0xffffffffu, (key_first + i * kBN + lane) % a.stride == 0);
+                            if (lane == 0) reinterpret_cast<uint32_t*>(sa - w32 + 3 * kBN)[part] = m;
                         }
-                        if (a.stride > 0) {                                               // landmark bits of the tile's keys
-                            const uint32_t m0 = __ballot_sync(0xffffffffu, (key0 + lane) % a.stride == 0);
-                            const uint32_t m1 = __ballot_sync(0xffffffffu, (key0 + 32 + lane) % a.stride == 0);
-                            if (lane == 0) {
-                                uint32_t* marks = reinterpret_cast<uint32_t*>(sa + 3 * kBN) + 2 * (warp & 1);
-                                marks[0] = m0;
-                                marks[1] = m1;
-                            }
-                            __syncwarp();
-                        }
-                        mbar_arrive(bar(SCFULL + sc));
+                        arrive_w(bar(SCFULL + sc));
+                        fetch_scales(i + 1);
                     }
                     const int st = n_t % ST;
-                    if (n_t >= ST && !__all_sync(0xffffffffu, mbar_wait(bar(EMPTY + st), ((n_t / ST) - 1) & 1, abort_flag))) { ok = false; break; }
-                    unsigned char* tile = tiles + st * C::kTile + (c16 >> 2) * 16384;
+                    if (n_t >= ST && !wait_w(bar(EMPTY + st), ((n_t / ST) - 1) & 1)) { ok = false; break; }
+                    unsigned char* tile = tiles + st * C::kTile + (c16 >> 2) * 16384 + (w32 + r16) * 128;
+#pragma unroll 1
+                    for (int blk = 0; blk < PPT; ++blk) {
+                        fetch(PPT * i + blk + C::kDepth - 1);
+                        cp_async_wait<C::kDepth - 1>();
+                        const unsigned char* in = raw + slot_out * 1024;
+                        slot_out = slot_out + 1 == C::kDepth ? 0 : slot_out + 1;
+                        uint4 xs[NP];
 #pragma unroll
-                    for (int u = 0; u < NI; ++u) {
-                        const int r = w64 + RI * u + lane / LR;
-                        const uint32_t w[4] = {buf[u].x ^ 0x80808080u, buf[u].y ^ 0x80808080u, buf[u].z ^ 0x80808080u, buf[u].w ^ 0x80808080u};
-                        unsigned char* row = tile + r * 128;
-                        const int ch = 2 * (c16 & 3);
-                        *reinterpret_cast<uint4*>(row + ((ch ^ (r & 7)) << 4)) =
-                            make_uint4(bytes_to_half2(w[0], 0x4140), bytes_to_half2(w[0], 0x4342), bytes_to_half2(w[1], 0x4140), bytes_to_half2(w[1], 0x4342));
-                        *reinterpret_cast<uint4*>(row + (((ch + 1) ^ (r & 7)) << 4)) =
-                            make_uint4(bytes_to_half2(w[2], 0x4140), bytes_to_half2(w[2], 0x4342), bytes_to_half2(w[3], 0x4140), bytes_to_half2(w[3], 0x4342));
+                        for (int u = 0; u < NP; ++u) xs[u] = *reinterpret_cast<const uint4*>(in + u * 512);
+#pragma unroll
+                        for (int u = 0; u < NP; ++u) {
+                            const uint4 x = xs[u];
+                            unsigned char* row = tile + (PR * blk + RI * u) * 128;
+                            const int sw = (RI * u + r16) & 7;        // PR blk and w32 are multiples of 8
+                            uint4 y0, y1;
+                            if (bf16) {
+                                y0 = make_uint4(bytes_to_bf162(x.x, 0x4140), bytes_to_bf162(x.x, 0x4342), bytes_to_bf162(x.y, 0x4140), bytes_to_bf162(x.y, 0x4342));
+                                y1 = make_uint4(bytes_to_bf162(x.z, 0x4140), bytes_to_bf162(x.z, 0x4342), bytes_to_bf162(x.w, 0x4140), bytes_to_bf162(x.w, 0x4342));
+                            } else {
+                                const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+                                y0 = make_uint4(bytes_to_half2(w[0], 0x4140), bytes_to_half2(w[0], 0x4342), bytes_to_half2(w[1], 0x4140), bytes_to_half2(w[1], 0x4342));
+                                y1 = make_uint4(bytes_to_half2(w[2], 0x4140), bytes_to_half2(w[2], 0x4342), bytes_to_half2(w[3], 0x4140), bytes_to_half2(w[3], 0x4342));
+                            }
+                            *reinterpret_cast<uint4*>(row + ((ch ^ sw) << 4)) = y0;
+                            *reinterpret_cast<uint4*>(row + (((ch + 1) ^ sw) << 4)) = y1;
+                        }
                     }
-                    load_tile(i + 1);
                     fence_async_smem();
-                    mbar_arrive(bar(FULL + st));
+                    arrive_w(bar(FULL + st));
                 }
+                cp_async_wait<0>();                                   // nothing of this segment is left in flight
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         if (work) {
-            // ================= softmax: one thread per query row =================
-            const int g = warp >> 2, r = (warp & 3) * 32 + lane;
-            const uint32_t lane_addr = ((uint32_t)((warp & 3) * 32)) << 16;
+            // ================= softmax: 16 query rows a warp =================
+            // A thread holds a quarter of two rows: slot q is row 8 q + lane / 4 of the warp, columns 2 (lane % 4), + 1 of every
+            // eight.  So it needs the three numbers of a quarter of the keys (shared memory returns 128 bytes a clock, broadcast
+            // or not), and four warps share a scheduler.
+            const int g = warp >> 3, quad = lane >> 2, col = 2 * (lane & 3);
+            const int wr = 32 * (warp & 3) + 16 * ((warp >> 2) & 1);         // the warp's first row of the tile, and TMEM lane
+            const uint32_t lane_addr = (uint32_t)wr << 16;
             const uint32_t tmem_S = tmem + (uint32_t)g * 128u + lane_addr, tmem_O = tmem + C::kColO + (uint32_t)(g * D) + lane_addr;
-            const uint32_t tmem_P = C::kOwnP ? tmem + C::kColP + (uint32_t)g * 64u + lane_addr : tmem_S;
-            // the TMEM accesses below are the whole warp's: so are the verdicts of its waits
-            auto wait_w = [&](uint32_t bb, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bb, parity, abort_flag)) != 0; };
+            const uint32_t tmem_P = C::kOwnP ? tmem + C::kColP + (uint32_t)g * 64u + lane_addr : tmem_S + 64u;
+            // the TMEM accesses below are the whole warp's: so are the verdicts of its waits, and its arrivals
+            auto wait_w = [&](uint32_t bb, uint32_t parity) { return wait_warp(bb, parity, abort_flag); };
+            auto arrive_w = [&](uint32_t bb) { __syncwarp(); if (lane == 0) mbar_arrive(bb); };
             int n_t = 0, s_run = 0;                   // key tiles seen, score tiles of this row tile taken
             bool ok = true;
             for (int n_seg = 0; ok; ++n_seg) {
                 const int sst = n_seg % kSegStages;
                 if (!wait_w(bar(SEGFULL + sst), (n_seg / kSegStages) & 1)) break;
-                const Segment sg = *reinterpret_cast<const Segment*>(smem + C::kOffSeg + sst * 64);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(SEGEMPTY + sst));
-                if (sg.n_iter == 0) break;
-                PagedSeq s; s.q0 = sg.q0; s.n = sg.n; s.kv = sg.kv; s.ok = true;
-                const int r0 = sg.row0 + 128 * g, row = r0 + r;
-                const bool live = row < sg.n_rows;
-                const int token = (live ? row : sg.row0) / a.G, head = sg.h * a.G + (live ? row : sg.row0) % a.G;
-                const int pos = sg.kv - sg.n + token;
-                int lo = 0, hi = 0, first = 0, last = 0;
-                if (r0 < sg.n_rows) {
-                    const int rows = min(128, sg.n_rows - r0);
-                    const Item mine = item_keys(a, s, r0, rows);
-                    lo = (mine.begin - sg.begin) / kBN;
-                    hi = (mine.end - sg.begin + kBN - 1) / kBN;
-                    first = sg.kv - sg.n + r0 / a.G;
-                    last = sg.kv - sg.n + (r0 + rows - 1) / a.G;
-                }
-                const bool shun = shunyam_active(a.window, sg.kv);
-                // the row into shared memory as FP16 times a power of two (its products so far are all done)
-                float alpha;
+                // The segment stays where it is, and its slot this warp's, until its output is written: its fields are read when they
+                // are wanted and hold no registers meanwhile.
+                const volatile Segment* seg = reinterpret_cast<const volatile Segment*>(smem + C::kOffSeg + sst * 64);
+                if (seg->n_iter == 0) break;
+                int lo = 0, hi = 0;                   // tiles of the item that this row tile takes part in
+                int e_hi = 0x7fffffff, e_lo = -0x7fffffff;   // a tile whose first key lies outside [e_lo, e_hi] is masked in part
                 {
-                    uint4 w[D / 8];
-                    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(sg.q0 + token) * a.q_row + (long long)head * a.q_head;
-                    float top = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) w[i] = live ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
-                    auto wide = [&](uint32_t x) {
-                        return a.is_f16 ? __half22float2(*reinterpret_cast<const __half2*>(&x)) : make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-                    };
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) { const float2 f = wide(ww[e]); top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y))); }
+                    const int n_rows = seg->n_rows, r0 = seg->row0 + 128 * g;
+                    if (r0 < n_rows) {
+                        PagedSeq s; s.q0 = seg->q0; s.n = seg->n; s.kv = seg->kv; s.ok = true;
+                        const int rows = min(128, n_rows - r0), begin = seg->begin;
+                        const Item mine = item_keys(a, s, r0, rows);
+                        lo = (mine.begin - begin) / kBN;
+                        hi = (mine.end - begin + kBN - 1) / kBN;
+                        const bool shun = shunyam_active(a.window, s.kv);
+                        if (a.causal || shun) e_hi = s.kv - s.n + r0 / a.G - (kBN - 1);
+                        if (shun) e_lo = s.kv - s.n + (r0 + rows - 1) / a.G - a.window;
                     }
-                    float mul;
-                    row_power(top, mul, alpha);
+                }
+                // the warp's rows into shared memory as they are, half a row a thread (the products so far are all done)
+                {
+                    const int r = wr + (lane >> 1), row0 = seg->row0, row = row0 + 128 * g + r;
+                    const bool live = row < seg->n_rows;
+                    const int token = (live ? row : row0) / a.G, head = seg->h * a.G + (live ? row : row0) % a.G;
+                    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(seg->q0 + token) * a.q_row + (long long)head * a.q_head;
                     unsigned char* dst = smem + C::kOffQ + g * C::kTile + r * 128;
+                    constexpr int N = D / 16;
+                    const int i0 = (lane & 1) * N;
+                    uint4 w[N];
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-                        uint32_t h[4];
+                    for (int i = 0; i < N; ++i) w[i] = live ? *reinterpret_cast<const uint4*>(src + 8 * (i0 + i)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) { const float2 f = wide(ww[e]); h[e] = f32x2_to_16(f.x * mul, f.y * mul, true); }
-                        *reinterpret_cast<uint4*>(dst + (i >> 3) * 16384 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-                    }
+                    for (int i = 0; i < N; ++i) *reinterpret_cast<uint4*>(dst + ((i0 + i) >> 3) * 16384 + ((((i0 + i) & 7) ^ (r & 7)) << 4)) = w[i];
                 }
                 fence_async_smem();
-                mbar_arrive(bar(QREADY + g));
+                arrive_w(bar(QREADY + g));
 
-                float m_run = -INFINITY, l_run = 0.0f;
-                int taken = 0;
-                for (int i = sg.i0; ok && i < sg.i0 + sg.n_iter; ++i, ++n_t) {
+                float2 nm[2], l_run[2];               // minus the row's reference, twice; its sum over even and odd keys
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    nm[q] = make_float2(-kNoReference, -kNoReference);
+                    l_run[q] = make_float2(0.0f, 0.0f);
+                }
+                bool first = true;                    // no tile taken yet
+                int i = seg->i0;
+                const int i_end = i + seg->n_iter;
+                int k0 = seg->begin + i * kBN;
+                for (; ok && i < i_end; ++i, ++n_t, k0 += kBN) {
                     const int sc = n_t % kScaleStages;
                     if (!wait_w(bar(SCFULL + sc), (n_t / kScaleStages) & 1)) { ok = false; break; }
-                    if (i < lo || i >= hi) { mbar_arrive(bar(SCEMPTY + sc)); continue; }
-                    const float* sa = reinterpret_cast<const float*>(smem + C::kOffScale + sc * C::kScaleBytes);
+                    if (i < lo || i >= hi) { arrive_w(bar(SCEMPTY + sc)); continue; }
+                    const float* sa = reinterpret_cast<const float*>(smem + C::kOffScale + sc * C::kScaleBytes) + col;
                     if (!wait_w(bar(SFULL + g), s_run & 1)) { ok = false; break; }
                     tc_fence_after();
-                    float x[kBN];
-                    tc_ld32(tmem_S, x);
-                    tc_ld32(tmem_S + 32, x + 32);
-                    tc_ld32(tmem_S + 64, x + 64);
-                    tc_ld32(tmem_S + 96, x + 96);
-                    tc_wait_ld();
-                    if (C::kOwnP) {                   // the next scores may overwrite these columns
-                        tc_fence_before();
-                        mbar_arrive(bar(SEMPTY + g));
-                    }
-                    const float2 al2 = make_float2(alpha, alpha);
-                    const float4* a4 = reinterpret_cast<const float4*>(sa);
-                    const float4* b4 = reinterpret_cast<const float4*>(sa + kBN);
-#pragma unroll
-                    for (int j = 0; j < kBN / 4; ++j) {
-                        const float4 ka = a4[j], kb = b4[j];
-                        const float2 f0 = __fmul2_rn(make_float2(ka.x, ka.y), al2), f1 = __fmul2_rn(make_float2(ka.z, ka.w), al2);
-                        const float2 y0 = __ffma2_rn(make_float2(x[4 * j], x[4 * j + 1]), f0, make_float2(kb.x, kb.y));
-                        const float2 y1 = __ffma2_rn(make_float2(x[4 * j + 2], x[4 * j + 3]), f1, make_float2(kb.z, kb.w));
-                        x[4 * j] = y0.x; x[4 * j + 1] = y0.y; x[4 * j + 2] = y1.x; x[4 * j + 3] = y1.y;
-                    }
-                    const int k0 = sg.begin + i * kBN;
-                    if ((a.causal && k0 + kBN - 1 > first) || (shun && k0 < last - a.window) || (shun && k0 + kBN - 1 > first)) {
-                        const uint32_t* marks = reinterpret_cast<const uint32_t*>(sa + 3 * kBN);
-                        const int top = pos - k0, low = shun ? pos - a.window - k0 : -1;       // window columns [low, top]
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int hi_q = top - 32 * q, lo_q = low - 32 * q;
-                            const uint32_t upto = hi_q < 0 ? 0u : hi_q >= 31 ? 0xffffffffu : (2u << hi_q) - 1u;
-                            const uint32_t from = lo_q <= 0 ? 0xffffffffu : lo_q > 31 ? 0u : 0xffffffffu << lo_q;
-                            uint32_t vis = (a.causal || shun) ? upto : 0xffffffffu;
-                            if (shun) {
-                                vis &= from;
-                                if (a.stride > 0) vis |= marks[q] & (a.causal ? upto : 0xffffffffu);
-                            }
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (!(vis & (1u << j))) x[32 * q + j] = -INFINITY;
-                        }
-                    }
-                    float mx;
-                    {
-                        float mc[8];
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) mc[q] = fmaxf(x[2 * q], x[2 * q + 1]);
-#pragma unroll
-                        for (int j = 16; j < kBN; j += 16)
-#pragma unroll
-                            for (int q = 0; q < 8; ++q) mc[q] = fmaxf(fmaxf(mc[q], x[j + 2 * q]), x[j + 2 * q + 1]);
-                        mx = fmaxf(fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])), fmaxf(fmaxf(mc[4], mc[5]), fmaxf(mc[6], mc[7])));
-                    }
-                    // the reference moves only when a weight would pass 2^8; the correction of O is warp-wide (TMEM access)
-                    const bool want = mx > m_run + kMoveMax || (m_run == -INFINITY && mx > -INFINITY);
-                    const bool any = __any_sync(0xffffffffu, want && taken > 0 && m_run > -INFINITY);
-                    float m_new = want ? mx : m_run;
-                    if (any && m_new < mx) m_new = mx;
-                    bool pv_done = taken == 0 || !C::kOwnP;       // without columns of its own, P's S came behind the last PV
-                    if (any) {
-                        if (!pv_done && !wait_w(bar(PVDONE + g), (s_run - 1) & 1)) { ok = false; break; }
-                        pv_done = true;
-                        tc_fence_after();
-                        const float f = m_run == -INFINITY ? 0.0f : ex2(m_run - m_new);
-#pragma unroll
-                        for (int hc = 0; hc < D / 16; ++hc) {
-                            float o[16];
-                            tc_ld16(tmem_O + 16 * hc, o);
+                    if (k0 > e_hi || k0 < e_lo) {
+                        // Some rows do not see some of the keys: -inf on their scores, in tensor memory, before the loop below.
+                        // (Inside it the test and the code would cost every tile registers and instruction fetches.)
+                        const uint32_t* marks = reinterpret_cast<const uint32_t*>(sa - col + 3 * kBN);
+                        const int pos0 = seg->kv - seg->n, row = seg->row0 + 128 * g + wr + quad;
+                        const int p0 = pos0 + row / a.G - k0 - col, p1 = pos0 + (row + 8) / a.G - k0 - col;
+                        const bool shun = shunyam_active(a.window, seg->kv), bounded = a.causal || shun;
+#pragma unroll 1
+                        for (int cb = 0; cb < kBN / 32; ++cb) {
+                            float y[16];
+                            tc_ld_16x256_x4(tmem_S + 32 * cb, y);
                             tc_wait_ld();
-                            uint32_t ow[16];
+                            const uint32_t m = a.stride > 0 ? marks[cb] >> col : 0u;
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) ow[j] = __float_as_uint(m_run == -INFINITY ? 0.0f : o[j] * f);
-                            tc_st8(tmem_O + 16 * hc, ow);
-                            tc_st8(tmem_O + 16 * hc + 8, ow + 8);
+                            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const int c = 32 * cb + 8 * w + e;
+                                    const bool mark = shun && ((m >> (8 * w + e)) & 1u);
+                                    const bool v0 = (!bounded || c <= p0) && (!shun || c >= p0 - a.window), v1 = (!bounded || c <= p1) && (!shun || c >= p1 - a.window);
+                                    if (!(v0 || (mark && (!a.causal || c <= p0)))) y[4 * w + e] = -INFINITY;
+                                    if (!(v1 || (mark && (!a.causal || c <= p1)))) y[4 * w + 2 + e] = -INFINITY;
+                                }
+                            tc_st_16x256_x4(tmem_S + 32 * cb, y);
                         }
                         tc_wait_st();
-                        tc_fence_before();
-                        l_run *= f;
                     }
-                    m_run = m_new;
-                    const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
-                    const float2 nm2 = make_float2(neg_m, neg_m);
-                    const float4* c4 = reinterpret_cast<const float4*>(sa + 2 * kBN);
-                    float2 la = make_float2(0.0f, 0.0f), lb = make_float2(0.0f, 0.0f);
-                    if (!pv_done) {                   // the last PV still reads P's columns until it is done
-                        if (!wait_w(bar(PVDONE + g), (s_run - 1) & 1)) { ok = false; break; }
-                        tc_fence_after();
-                    }
+                    bool pv_done = first || !C::kOwnP;       // without columns of its own, P's S came behind the last PV
+                    float x[kBW / 2];                 // [4 (key / 8) + 2 slot + column]
+                    ld_scores(tmem_S + kBN - kBW, x);
+                    // Blocks of kBW keys, highest first (P may lie on the S of the blocks before).  The loop stays rolled, and
+                    // nothing in it waits for a maximum: a weight's exponent is taken against the row's reference, and only when
+                    // one passes 2^15 -- or the row has no reference yet -- does the warp turn aside to move it.
+#pragma unroll 1
+                    for (int cb = kBN / kBW - 1; cb >= 0; --cb) {
+                        const float* sk = sa + kBW * cb;
+                        float z[kBW / 2];
+                        tc_wait_ld();
 #pragma unroll
-                    for (int cb = 0; cb < kBN / 16; ++cb) {
-                        uint32_t pk[8];
+                        for (int w = 0; w < kBW / 8; ++w) {
+                            const float2 ka = *reinterpret_cast<const float2*>(sk + 8 * w), kb = *reinterpret_cast<const float2*>(sk + kBN + 8 * w);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int j = 16 * cb + 4 * e;
-                            const float2 t0 = __fadd2_rn(make_float2(x[j], x[j + 1]), nm2), t1 = __fadd2_rn(make_float2(x[j + 2], x[j + 3]), nm2);
-                            const float2 p0 = make_float2(ex2(t0.x), ex2(t0.y)), p1 = make_float2(ex2(t1.x), ex2(t1.y));
-                            const float4 ci = c4[j / 4];
-                            la = __ffma2_rn(p0, make_float2(ci.x, ci.y), la);
-                            lb = __ffma2_rn(p1, make_float2(ci.z, ci.w), lb);
-                            pk[2 * e] = f32x2_to_16(p0.x, p0.y, true);
-                            pk[2 * e + 1] = f32x2_to_16(p1.x, p1.y, true);
+                            for (int q = 0; q < 2; ++q) {
+                                const int at = 4 * w + 2 * q;
+                                const float2 t = __ffma2_rn(make_float2(x[at], x[at + 1]), ka, __fadd2_rn(kb, nm[q]));
+                                z[at] = t.x;
+                                z[at + 1] = t.y;
+                            }
                         }
-                        tc_st8(tmem_P + 8 * cb, pk);
+                        float t0 = fmaxf(z[0], z[1]), t1 = fmaxf(z[2], z[3]);
+#pragma unroll
+                        for (int j = 4; j < kBW / 2; j += 4) {
+                            t0 = fmaxf(fmaxf(t0, z[j]), z[j + 1]);
+                            t1 = fmaxf(fmaxf(t1, z[j + 2]), z[j + 3]);
+                        }
+                        if (__builtin_expect(__any_sync(0xffffffffu, fmaxf(t0, t1) > kMoveMax), 0)) {
+                            // Move the references of the rows that outgrew theirs to the largest exponent of the block, and scale
+                            // what was summed against the old ones: l, O, and the blocks of P that this tile already has.
+                            float y[kBW / 2], f[2];                    // the scores again: z lost them to a reference of -1e30
+                            ld_scores(tmem_S + kBW * cb, y);
+                            tc_wait_ld();
+                            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                            for (int w = 0; w < kBW / 8; ++w) {
+                                const float2 ka = *reinterpret_cast<const float2*>(sk + 8 * w), kb = *reinterpret_cast<const float2*>(sk + kBN + 8 * w);
+#pragma unroll
+                                for (int q = 0; q < 2; ++q) {
+                                    const int at = 4 * w + 2 * q;
+                                    const float2 t = __ffma2_rn(make_float2(y[at], y[at + 1]), ka, kb);
+                                    y[at] = z[at] == -INFINITY ? -INFINITY : t.x;
+                                    y[at + 1] = z[at + 1] == -INFINITY ? -INFINITY : t.y;
+                                    top[q] = fmaxf(top[q], fmaxf(y[at], y[at + 1]));
+                                }
+                            }
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 1));
+                                // a whole number: the scaling by 2^-whole below is exact, in FP16 too
+                                top[q] = ceilf(fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 2)));
+                                const bool move = top[q] + nm[q].x > kMoveMax;
+                                f[q] = !move ? 1.0f : nm[q].x == -kNoReference ? 0.0f : ex2(-nm[q].x - top[q]);
+                                if (move) {
+                                    nm[q] = make_float2(-top[q], -top[q]);
+#pragma unroll
+                                    for (int w = 0; w < kBW / 8; ++w) {
+                                        z[4 * w + 2 * q] = y[4 * w + 2 * q] - top[q];
+                                        z[4 * w + 2 * q + 1] = y[4 * w + 2 * q + 1] - top[q];
+                                    }
+                                }
+                                l_run[q] = __fmul2_rn(l_run[q], make_float2(f[q], f[q]));
+                            }
+                            if (!first) {
+                                if (!pv_done && !wait_w(bar(PVDONE + g), (s_run - 1) & 1)) { ok = false; break; }
+                                pv_done = true;
+                                tc_fence_after();
+                                float o[16];
+#pragma unroll 1
+                                for (int hc = 0; hc < D / 32; ++hc) {
+                                    tc_ld_16x256_x4(tmem_O + 32 * hc, o);
+                                    tc_wait_ld();
+#pragma unroll
+                                    for (int j = 0; j < 16; ++j) o[j] *= f[(j >> 1) & 1];
+                                    tc_st_16x256_x4(tmem_O + 32 * hc, o);
+                                }
+                            }
+                            tc_wait_st();
+#pragma unroll 1
+                            for (int done = (kBW / 32) * (cb + 1); done < kBN / 32; ++done) {
+                                uint32_t pw[8];
+                                tc_ld_16x128_x4(tmem_P + 16 * done, pw);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&pw[j]), __float2half2_rn(f[j & 1]));
+                                    pw[j] = *reinterpret_cast<const uint32_t*>(&h);
+                                }
+                                tc_st_16x128_x4(tmem_P + 16 * done, pw);
+                            }
+                            tc_wait_st();
+                            tc_fence_before();
+                        }
+                        if (cb > 0) {                 // the next block's scores, under this one's exponentials
+                            ld_scores(tmem_S + kBW * (cb - 1), x);
+                        } else if (C::kOwnP) {        // all scores have left: the next ones may overwrite these columns
+                            tc_fence_before();
+                            arrive_w(bar(SEMPTY + g));
+                        }
+                        if (!pv_done) {               // the last PV still reads P's columns until it is done
+                            if (!wait_w(bar(PVDONE + g), (s_run - 1) & 1)) { ok = false; break; }
+                            pv_done = true;
+                            tc_fence_after();
+                        }
+#pragma unroll
+                        for (int part = kBW / 32 - 1; part >= 0; --part) {
+                            uint32_t pk[8];
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                const float2 ci = *reinterpret_cast<const float2*>(sk + 2 * kBN + 32 * part + 8 * w);
+#pragma unroll
+                                for (int q = 0; q < 2; ++q) {
+                                    const int at = 16 * part + 4 * w + 2 * q;
+                                    const float2 pw = make_float2(ex2(z[at]), ex2(z[at + 1]));
+                                    l_run[q] = __ffma2_rn(pw, ci, l_run[q]);
+                                    pk[2 * w + q] = f32x2_to_16(pw.x, pw.y, true);
+                                }
+                            }
+                            tc_st_16x128_x4(tmem_P + (kBW / 2) * cb + 16 * part, pk);
+                        }
                     }
-                    mbar_arrive(bar(SCEMPTY + sc));
-                    l_run += (la.x + la.y) + (lb.x + lb.y);
+                    if (!ok) break;
+                    arrive_w(bar(SCEMPTY + sc));
                     tc_wait_st();
                     tc_fence_before();
-                    mbar_arrive(bar(PFULL + g));
+                    arrive_w(bar(PFULL + g));
                     ++s_run;
-                    ++taken;
+                    first = false;
                 }
                 if (!ok) break;
-                // ---- the segment's result: an output row, or a partial one ----
-                if (taken > 0) {
+                // ---- the segment's result: output rows, or partial ones ----
+                if (!first) {
                     if (!wait_w(bar(PVDONE + g), (s_run - 1) & 1)) break;
                     tc_fence_after();
                 }
-                if (m_run == -INFINITY && !(l_run == 0.0f)) m_run = 0.0f;      // scores that are all NaN: not an empty row
-                const bool empty = taken == 0 || m_run == -INFINITY;
-                const size_t rec = (size_t)(sg.slot < 0 ? 0 : sg.slot) * kChunkRows + 128 * g + r;
-                if (sg.slot >= 0 && live) a.stat[rec] = make_float2(empty ? -INFINITY : m_run, l_run);
-                const float inv = empty ? 0.0f : 1.0f / l_run;
+                const int slot = seg->slot;
+                float inv[2];
+                bool live[2], empty[2];
+                size_t rec[2];
+                uint16_t* dst[2];
 #pragma unroll
-                for (int hc = 0; hc < D / 16; ++hc) {
+                for (int q = 0; q < 2; ++q) {
+                    float l = l_run[q].x + l_run[q].y;
+                    l += __shfl_xor_sync(0xffffffffu, l, 1);
+                    l += __shfl_xor_sync(0xffffffffu, l, 2);
+                    const float m = -nm[q].x;
+                    empty[q] = first || (m == kNoReference && l == 0.0f);   // (scores that are all NaN leave l NaN)
+                    inv[q] = empty[q] ? 0.0f : slot >= 0 ? 1.0f : 1.0f / l;
+                    const int r = wr + 8 * q + quad, row = seg->row0 + 128 * g + r;
+                    live[q] = row < seg->n_rows;
+                    rec[q] = (size_t)(slot < 0 ? 0 : slot) * kChunkRows + 128 * g + r;
+                    dst[q] = static_cast<uint16_t*>(a.o) + (long long)(seg->q0 + row / a.G) * a.o_row + (long long)(seg->h * a.G + row % a.G) * a.o_head + col;
+                    if (slot >= 0 && live[q] && col == 0) a.stat[rec[q]] = make_float2(empty[q] ? -INFINITY : m, l);
+                }
+#pragma unroll 1
+                for (int hc = 0; hc < D / 32; ++hc) {
                     float o[16];
                     __syncwarp();
-                    if (taken > 0) {                  // warp-uniform: the row tile took part
-                        tc_ld16(tmem_O + 16 * hc, o);
+                    if (!first) {                     // warp-uniform: the row tile took part
+                        tc_ld_16x256_x4(tmem_O + 32 * hc, o);
                         tc_wait_ld();
                     }
-                    if (!live) continue;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) o[j] = empty ? 0.0f : o[j];
-                    if (sg.slot >= 0) {
-                        float4* dst = reinterpret_cast<float4*>(a.part + rec * D + 16 * hc);
+                    for (int w = 0; w < 4; ++w)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                    } else {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) w[j] = f32x2_to_16(o[2 * j] * inv, o[2 * j + 1] * inv, a.is_f16 != 0);
-                        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + (long long)(sg.q0 + token) * a.o_row + (long long)head * a.o_head + 16 * hc);
-                        dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                        dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-                    }
+                        for (int q = 0; q < 2; ++q) {
+                            const float y0 = empty[q] ? 0.0f : o[4 * w + 2 * q] * inv[q], y1 = empty[q] ? 0.0f : o[4 * w + 2 * q + 1] * inv[q];
+                            if (!live[q]) continue;
+                            if (slot >= 0) *reinterpret_cast<float2*>(a.part + rec[q] * D + 32 * hc + 8 * w + col) = make_float2(y0, y1);
+                            else *reinterpret_cast<uint32_t*>(dst[q] + 32 * hc + 8 * w) = f32x2_to_16(y0, y1, a.is_f16 != 0);
+                        }
                 }
                 tc_fence_before();
+                arrive_w(bar(SEGEMPTY + sst));
             }
         }
     }
