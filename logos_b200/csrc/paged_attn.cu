@@ -13,8 +13,9 @@
 // fragments come straight from global memory: S = q K^T has the rows as M and the keys as N, O^T = V^T p has the
 // channels as M and the rows as N, and the accumulator of the first is the B operand of the second as it is, so p
 // never moves between threads.  The order of the channels inside a product is free, so a thread's share of a K row is
-// 16 consecutive bytes and its share of a V row DH / 8: every load is a wide one and nothing is staged in shared
-// memory.  (tcgen05 needs 128 rows to be busy and its operands in shared memory; here a head has 1 to 16.)
+// 16 consecutive bytes and its share of a V row DH / 8.  Blocks of 2 KiB of K and 2 KiB of V and their scales come by
+// cp.async.bulk -- a head's rows of a page are contiguous -- into a ring of each warp's own, filled by one of its lanes
+// and awaited by the warp alone: kStages blocks in flight, and no registers or instructions spent on them.  (tcgen05 needs 128 rows to be busy and its operands in shared memory; here a head has 1 to 16.)
 // int8 -> FP16 costs five instructions for four values: bytes biased to unsigned, spliced under the exponent of 1024
 // and the bias subtracted.
 //
@@ -22,12 +23,14 @@
 // blocks in turn, each with its own running maximum, and join in shared memory.  Chunks join through the workspace:
 // the last CTA to arrive sums the partial results in the order of the chunks.
 #include "paged.cuh"
+#include "tcgen05_ptx.cuh"
 
 namespace logos {
 namespace {
 
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = 32 * kSplitWarps;
+constexpr int kStages = 3;                       // blocks in a warp's ring
 constexpr int kSpan = 2048;                      // keys whose pages a warp's lanes hold, one 16-key block each
 constexpr int kFewRows = 32;                     // query rows per head up to which a sequence is this kernel's
 constexpr int kSplitCounters = (int)(kWorkspaceCounterBytes / sizeof(int));
@@ -63,15 +66,44 @@ __device__ __forceinline__ void store_out(const SplitArgs& a, int token, int hea
     else *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.o) + at) = __floats2bfloat162_rn(x, y);
 }
 
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// a warp's bounded wait for one of its blocks
+__device__ __forceinline__ bool wait_block(uint32_t bar, uint32_t parity) {
+    for (uint32_t it = 0; it < (1u << 18); ++it) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+
+// shared memory of a CTA: the warps' rings, their barriers; the join of the warps uses the rings' space
+template <int D, int NQ> struct SplitShape {
+    static constexpr int kRows = 8 * NQ, kKB = 2048 / D;      // keys of a block
+    static constexpr int kOffV = 2048, kOffKs = 4096, kOffVs = kOffKs + 4 * kKB, kStage = kOffVs + 4 * kKB;
+    static constexpr int kRings = kSplitWarps * kStages * kStage;
+    static constexpr int kPitch = D + 4;
+    static constexpr int kJoin = kSplitWarps * kRows * (kPitch + 2) * 4;
+    static constexpr int kOffBar = kRings > kJoin ? kRings : kJoin;
+    static constexpr int kSmem = kOffBar + 8 * kSplitWarps * kStages;
+};
+
 // NQ: groups of 8 query rows in the tile
 template <int D, int NQ>
 __global__ void __launch_bounds__(kSplitThreads)
 paged_split_kernel(const __grid_constant__ SplitArgs a) {
-    constexpr int ROWS = 8 * NQ, KB = 2048 / D;  // keys of a block: 2 KiB of K and 2 KiB of V in a warp's registers
+    using C = SplitShape<D, NQ>;
+    constexpr int ROWS = C::kRows, KB = C::kKB, SUB = KB / 16;   // SUB: 16-key pieces of a block
     constexpr int KG = KB / 8, KS = D / 16, MT = D / 16, VW = D / 32;   // key groups; k steps of S; channel tiles; words of a V share
-    constexpr int PITCH = D + 4;
-    __shared__ float s_o[kSplitWarps][ROWS][PITCH];
-    __shared__ float s_m[kSplitWarps][ROWS], s_l[kSplitWarps][ROWS];
+    constexpr int PITCH = C::kPitch;
+    extern __shared__ __align__(128) unsigned char smem[];
+    float (*s_o)[ROWS][PITCH] = reinterpret_cast<float (*)[ROWS][PITCH]>(smem);
+    float (*s_m)[ROWS] = reinterpret_cast<float (*)[ROWS]>(smem + kSplitWarps * ROWS * PITCH * 4);
+    float (*s_l)[ROWS] = s_m + kSplitWarps;
     __shared__ int s_last;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -96,11 +128,17 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
     if (split >= n_splits) return;
     const int c0 = k_begin + split * a.chunk, c1 = min(c0 + a.chunk, k_end);
 
+    // The warp's ring.  Lane 0 fills it; the barriers are this warp's alone.
+    unsigned char* ring = smem + warp * (kStages * C::kStage);
+    const uint32_t ring_addr = tc::smem_u32(ring), bar0 = tc::smem_u32(smem + C::kOffBar) + 8 * (warp * kStages);
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) tc::mbar_init(bar0 + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     // The chunk is walked in spans of 2048 keys.  Block i of a warp in a span is keys s0 + (4 i + warp) KB ...; lane
     // SUB i + j holds the page of its j-th 16 keys (a page never ends inside 16 keys).
     int s0 = c0, s1 = c0, n_iter = 0, my_page = -1;
     auto open_span = [&](int at0) {
-        constexpr int SUB = KB / 16;
         s0 = at0;
         s1 = min(s0 + kSpan, c1);
         n_iter = (s1 - s0 - warp * KB + kSplitWarps * KB - 1) / (kSplitWarps * KB);
@@ -112,53 +150,37 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
         }
     };
     open_span(c0);
-
-    uint4 kr[KG][D / 64];
-    uint32_t vr[KB / 4][VW];
-    float2 ksr[KG], vsr[KG];
-    // A page that is not there is read as page 0 and masked later: no load waits for a test.
-    auto load_k = [&](int it) {
+    int n_in = 0;                                 // blocks requested so far; block n lies in stage n % kStages
+    // Requests block `it` of the span.  A piece whose page is not there is left out: what its place in the ring holds is
+    // masked.  (The lanes have read the stage's last block: the __syncwarp before.)
+    auto request = [&](int it) {
         if (it >= n_iter) return;
+        const int st = n_in % kStages;
+        int page[SUB];
 #pragma unroll
-        for (int u2 = 0; u2 < KG / 2; ++u2) {
-            const int page = max(__shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + u2) & 31), 0);
-            const int key = s0 + (it * kSplitWarps + warp) * KB + 16 * u2;
-            const size_t row = paged_row(a.p, page, h) + (key & ((1 << a.p.page_shift) - 1));
-            const uint4* at = reinterpret_cast<const uint4*>(a.p.k + (row + g) * D) + t;
-            const float2* sk = reinterpret_cast<const float2*>(a.p.ks + row) + t;
-            const float2* sv = reinterpret_cast<const float2*>(a.p.vs + row) + t;
+        for (int j = 0; j < SUB; ++j) page[j] = __shfl_sync(0xffffffffu, my_page, (it * SUB + j) & 31);
+        if (lane == 0) {
+            const uint32_t dst = ring_addr + st * C::kStage, bar = bar0 + 8 * st;
+            const int key = s0 + (it * kSplitWarps + warp) * KB;
+            uint32_t bytes = 0;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int j = 0; j < SUB; ++j) bytes += page[j] >= 0 ? 16 * (2 * D + 8) : 0;
+            tc::mbar_expect_tx(bar, bytes);
 #pragma unroll
-                for (int i = 0; i < D / 64; ++i) kr[2 * u2 + e][i] = __ldg(at + 8 * e * (D / 16) + 4 * i);
-                ksr[2 * u2 + e] = __ldg(sk + 4 * e);
-                vsr[2 * u2 + e] = __ldg(sv + 4 * e);
+            for (int j = 0; j < SUB; ++j) {
+                if (page[j] < 0) continue;
+                const size_t row = paged_row(a.p, page[j], h) + ((key + 16 * j) & ((1 << a.p.page_shift) - 1));
+                bulk_load(dst + 16 * j * D, a.p.k + row * D, 16 * D, bar);
+                bulk_load(dst + C::kOffV + 16 * j * D, a.p.v + row * D, 16 * D, bar);
+                bulk_load(dst + C::kOffKs + 64 * j, a.p.ks + row, 64, bar);
+                bulk_load(dst + C::kOffVs + 64 * j, a.p.vs + row, 64, bar);
             }
         }
+        ++n_in;
     };
-    auto load_v = [&](int it) {
-        if (it >= n_iter) return;
-#pragma unroll
-        for (int u2 = 0; u2 < KG / 2; ++u2) {
-            const int page = max(__shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + u2) & 31), 0);
-            const int key = s0 + (it * kSplitWarps + warp) * KB + 16 * u2;
-            const size_t row = paged_row(a.p, page, h) + (key & ((1 << a.p.page_shift) - 1)) + 2 * t;
-            const int8_t* at = a.p.v + row * D + g * (D / 8);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {                // keys 2t, 2t + 1, 2t + 8, 2t + 9
-                const int8_t* w = at + (8 * (i >> 1) + (i & 1)) * D;
-                if (D == 64) {
-                    const uint2 x = __ldg(reinterpret_cast<const uint2*>(w));
-                    vr[4 * u2 + i][0] = x.x; vr[4 * u2 + i][1] = x.y;
-                } else {
-                    const uint4 x = __ldg(reinterpret_cast<const uint4*>(w));
-                    vr[4 * u2 + i][0] = x.x; vr[4 * u2 + i][1] = x.y; vr[4 * u2 + i][VW - 2] = x.z; vr[4 * u2 + i][VW - 1] = x.w;
-                }
-            }
-        }
-    };
-    load_k(0);
-    load_v(0);
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < kStages; ++i) request(i);
 
     // the rows' A fragments: k step 4 i + e of the products holds channels 64 i + 16 t + 4 e ... + 3 of this thread
     uint32_t qa[KS][4];
@@ -217,9 +239,13 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
             for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
     }
 
+    int n_out = 0;                                // blocks taken so far
+    bool ok = true;
     for (;;) {
-    for (int it = 0; it < n_iter; ++it) {
+    for (int it = 0; it < n_iter; ++it, ++n_out) {
         const int k0 = s0 + (it * kSplitWarps + warp) * KB;
+        const unsigned char* blk = ring + (n_out % kStages) * C::kStage;
+        ok = wait_block(bar0 + 8 * (n_out % kStages), (n_out / kStages) & 1) && ok;
         float sc[KG][4];
         float2 inv[KG];
         bool whole = true;                       // every key of the block is there
@@ -229,25 +255,26 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
             for (int e = 0; e < 4; ++e) sc[u][e] = 0.0f;
 #pragma unroll
             for (int i = 0; i < D / 64; ++i) {
-                const uint32_t w[4] = {kr[u][i].x ^ 0x80808080u, kr[u][i].y ^ 0x80808080u, kr[u][i].z ^ 0x80808080u, kr[u][i].w ^ 0x80808080u};
+                const uint4 kr = *reinterpret_cast<const uint4*>(blk + (8 * u + g) * D + 64 * i + 16 * t);
+                const uint32_t w[4] = {kr.x ^ 0x80808080u, kr.y ^ 0x80808080u, kr.z ^ 0x80808080u, kr.w ^ 0x80808080u};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mma_f16(sc[u], qa[4 * i + e], bytes_to_half2(w[e], 0x4140), bytes_to_half2(w[e], 0x4342));
             }
-            const float v0 = fmaxf(vsr[u].x, kLeastScale), v1 = fmaxf(vsr[u].y, kLeastScale);
+            const float2 ksr = *reinterpret_cast<const float2*>(blk + C::kOffKs + 32 * u + 8 * t), vsr = *reinterpret_cast<const float2*>(blk + C::kOffVs + 32 * u + 8 * t);
+            const float v0 = fmaxf(vsr.x, kLeastScale), v1 = fmaxf(vsr.y, kLeastScale);
             const float b0 = __log2f(v0), b1 = __log2f(v1);
             inv[u] = make_float2(__fdividef(1.0f, v0), __fdividef(1.0f, v1));
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                sc[u][2 * n] = fmaf(sc[u][2 * n], alpha[n] * ksr[u].x, b0);
-                sc[u][2 * n + 1] = fmaf(sc[u][2 * n + 1], alpha[n] * ksr[u].y, b1);
+                sc[u][2 * n] = fmaf(sc[u][2 * n], alpha[n] * ksr.x, b0);
+                sc[u][2 * n + 1] = fmaf(sc[u][2 * n + 1], alpha[n] * ksr.y, b1);
             }
-            whole = whole && __shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + (u >> 1)) & 31) >= 0;
+            whole = whole && __shfl_sync(0xffffffffu, my_page, (it * SUB + (u >> 1)) & 31) >= 0;
         }
-        load_k(it + 1);
         if (!whole || shun || k0 + KB > c1 || (a.causal && k0 + KB - 1 > first)) {
 #pragma unroll
             for (int u = 0; u < KG; ++u) {
-                const bool there = __shfl_sync(0xffffffffu, my_page, (it * (KB / 16) + (u >> 1)) & 31) >= 0;
+                const bool there = __shfl_sync(0xffffffffu, my_page, (it * SUB + (u >> 1)) & 31) >= 0;
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -296,11 +323,23 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
         }
         // O^T += V^T p: the thread's channels are g DH / 8 + 2 tile, + 1
 #pragma unroll
-        for (int u2 = 0; u2 < KG / 2; ++u2)
+        for (int u2 = 0; u2 < KG / 2; ++u2) {
+            uint32_t vr[4][VW];                  // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the 16
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned char* at = blk + C::kOffV + (16 * u2 + 2 * t + 8 * (i >> 1) + (i & 1)) * D + g * (D / 8);
+                if (D == 64) {
+                    const uint2 x = *reinterpret_cast<const uint2*>(at);
+                    vr[i][0] = x.x ^ 0x80808080u; vr[i][1] = x.y ^ 0x80808080u;
+                } else {
+                    const uint4 x = *reinterpret_cast<const uint4*>(at);
+                    vr[i][0] = x.x ^ 0x80808080u; vr[i][1] = x.y ^ 0x80808080u;
+                    vr[i][VW - 2] = x.z ^ 0x80808080u; vr[i][VW - 1] = x.w ^ 0x80808080u;
+                }
+            }
 #pragma unroll
             for (int w = 0; w < VW; ++w) {
-                const uint32_t x0 = vr[4 * u2][w] ^ 0x80808080u, x1 = vr[4 * u2 + 1][w] ^ 0x80808080u;
-                const uint32_t y0 = vr[4 * u2 + 2][w] ^ 0x80808080u, y1 = vr[4 * u2 + 3][w] ^ 0x80808080u;
+                const uint32_t x0 = vr[0][w], x1 = vr[1][w], y0 = vr[2][w], y1 = vr[3][w];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t mx = prmt(x0, x1, half ? 0x7362 : 0x5140), my = prmt(y0, y1, half ? 0x7362 : 0x5140);
@@ -310,13 +349,17 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
                     for (int n = 0; n < NQ; ++n) mma_f16(o[n][2 * w + half], va, pb[n][2 * u2], pb[n][2 * u2 + 1]);
                 }
             }
-        load_v(it + 1);
+        }
+        __syncwarp();                            // the block has been read by every lane
+        request(it + kStages);
     }
     if (s1 >= c1) break;
     open_span(s1);
-    load_k(0);
-    load_v(0);
+#pragma unroll 1
+    for (int i = 0; i < kStages; ++i) request(i);
     }
+    if (!ok && lane == 0) atomicCAS(a.p.status, 0, 0x40000000);
+    __syncthreads();                             // no block is on its way any more: the rings' space is free
 
     // join the warps: statistics of row 8 n + g, then the outputs scaled to the CTA's maximum
 #pragma unroll
@@ -420,13 +463,18 @@ SplitPlan plan_split(const logos_ctx* ctx, const logos_paged_cache* c, const log
     return p;
 }
 
-template <int D>
-int launch_split(logos_ctx* ctx, const SplitArgs& a, int rows) {
+template <int D, int NQ>
+int launch_split(logos_ctx* ctx, const SplitArgs& a) {
     const dim3 grid((unsigned)((int64_t)a.splits * a.p.H * a.tiles), a.p.B);
-    if (rows == 8) paged_split_kernel<D, 1><<<grid, kSplitThreads, 0, ctx->stream>>>(a);
-    else paged_split_kernel<D, 2><<<grid, kSplitThreads, 0, ctx->stream>>>(a);
+    auto* fn = paged_split_kernel<D, NQ>;
+    if (int rc = ensure_smem_limit(ctx, fn, SplitShape<D, NQ>::kSmem)) return rc;
+    fn<<<grid, kSplitThreads, SplitShape<D, NQ>::kSmem, ctx->stream>>>(a);
     LOGOS_LAUNCH_CHECK(ctx, "paged_split_kernel");
     return LOGOS_OK;
+}
+template <int D>
+int launch_split(logos_ctx* ctx, const SplitArgs& a, int rows) {
+    return rows == 8 ? launch_split<D, 1>(ctx, a) : launch_split<D, 2>(ctx, a);
 }
 
 }  // namespace
