@@ -70,6 +70,12 @@ __device__ __forceinline__ uint32_t bytes_to_bf162(uint32_t bytes, uint32_t sel)
     return *reinterpret_cast<uint32_t*>(&r);
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // A query row in FP16 by a power of two: `top` = max|q| of the row.  The factor puts it at 2^13 ... 2^14, so a BF16
 // row keeps every bit of values down to 2^-27 of its largest; rows of zeros, infinities or NaN keep factor 1.
 __device__ __forceinline__ void row_power(float top, float& mul, float& inv) {

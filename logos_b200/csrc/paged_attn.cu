@@ -14,8 +14,9 @@
 // channels as M and the rows as N, and the accumulator of the first is the B operand of the second as it is, so p
 // never moves between threads.  The order of the channels inside a product is free, so a thread's share of a K row is
 // 16 consecutive bytes and its share of a V row DH / 8.  Blocks of 2 KiB of K and 2 KiB of V and their scales come by
-// cp.async.bulk -- a head's rows of a page are contiguous -- into a ring of each warp's own, filled by one of its lanes
-// and awaited by the warp alone: kStages blocks in flight, and no registers or instructions spent on them.  (tcgen05 needs 128 rows to be busy and its operands in shared memory; here a head has 1 to 16.)
+// cp.async into a ring of each warp's own, kStages blocks in flight and no registers spent on them.  (By cp.async.bulk, one
+// lane for all, it took 80 instructions more a block, for the operands of its eight copies: 237 us where this takes 197, 64 sequences x
+// 16 heads x 8192 tokens.)  (tcgen05 needs 128 rows to be busy and its operands in shared memory; here a head has 1 to 16.)
 // int8 -> FP16 costs five instructions for four values: bytes biased to unsigned, spliced under the exponent of 1024
 // and the bias subtracted.
 //
@@ -23,14 +24,13 @@
 // blocks in turn, each with its own running maximum, and join in shared memory.  Chunks join through the workspace:
 // the last CTA to arrive sums the partial results in the order of the chunks.
 #include "paged.cuh"
-#include "tcgen05_ptx.cuh"
 
 namespace logos {
 namespace {
 
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = 32 * kSplitWarps;
-constexpr int kStages = 3;                       // blocks in a warp's ring
+constexpr int kStages = 2;                       // blocks in a warp's ring
 constexpr int kSpan = 2048;                      // keys whose pages a warp's lanes hold, one 16-key block each
 constexpr int kFewRows = 32;                     // query rows per head up to which a sequence is this kernel's
 constexpr int kSplitCounters = (int)(kWorkspaceCounterBytes / sizeof(int));
@@ -66,30 +66,15 @@ __device__ __forceinline__ void store_out(const SplitArgs& a, int token, int hea
     else *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.o) + at) = __floats2bfloat162_rn(x, y);
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-// a warp's bounded wait for one of its blocks
-__device__ __forceinline__ bool wait_block(uint32_t bar, uint32_t parity) {
-    for (uint32_t it = 0; it < (1u << 18); ++it) {
-        uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-        if (ok) return true;
-    }
-    return false;
-}
-
-// shared memory of a CTA: the warps' rings, their barriers; the join of the warps uses the rings' space
+// shared memory of a CTA: the warps' rings; the join of the warps uses their space
 template <int D, int NQ> struct SplitShape {
     static constexpr int kRows = 8 * NQ, kKB = 2048 / D;      // keys of a block
     static constexpr int kOffV = 2048, kOffKs = 4096, kOffVs = kOffKs + 4 * kKB, kStage = kOffVs + 4 * kKB;
-    static constexpr int kRings = kSplitWarps * kStages * kStage;
+    static constexpr int kScaled = 8 * kKB;                   // log2 vs and 1 / vs of the warp's current block
+    static constexpr int kRings = kSplitWarps * (kStages * kStage + kScaled);
     static constexpr int kPitch = D + 4;
     static constexpr int kJoin = kSplitWarps * kRows * (kPitch + 2) * 4;
-    static constexpr int kOffBar = kRings > kJoin ? kRings : kJoin;
-    static constexpr int kSmem = kOffBar + 8 * kSplitWarps * kStages;
+    static constexpr int kSmem = kRings > kJoin ? kRings : kJoin;
 };
 
 // NQ: groups of 8 query rows in the tile
@@ -128,16 +113,13 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
     if (split >= n_splits) return;
     const int c0 = k_begin + split * a.chunk, c1 = min(c0 + a.chunk, k_end);
 
-    // The warp's ring.  Lane 0 fills it; the barriers are this warp's alone.
-    unsigned char* ring = smem + warp * (kStages * C::kStage);
-    const uint32_t ring_addr = tc::smem_u32(ring), bar0 = tc::smem_u32(smem + C::kOffBar) + 8 * (warp * kStages);
-    if (lane == 0) {
-        for (int i = 0; i < kStages; ++i) tc::mbar_init(bar0 + 8 * i, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
+    unsigned char* ring = smem + warp * (kStages * C::kStage + C::kScaled);
+    float* scaled = reinterpret_cast<float*>(ring + kStages * C::kStage);
+    const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
     // The chunk is walked in spans of 2048 keys.  Block i of a warp in a span is keys s0 + (4 i + warp) KB ...; lane
     // SUB i + j holds the page of its j-th 16 keys (a page never ends inside 16 keys).
     int s0 = c0, s1 = c0, n_iter = 0, my_page = -1;
+    bool whole = true;                            // every page of the warp's blocks is there
     auto open_span = [&](int at0) {
         s0 = at0;
         s1 = min(s0 + kSpan, c1);
@@ -148,37 +130,33 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
             my_page = paged_page(a.p, b, at);
             if (my_page < 0) report_batch(a.p.status, b, true);
         }
+        whole = __all_sync(0xffffffffu, at >= s1 || my_page >= 0);
     };
     open_span(c0);
-    int n_in = 0;                                 // blocks requested so far; block n lies in stage n % kStages
-    // Requests block `it` of the span.  A piece whose page is not there is left out: what its place in the ring holds is
-    // masked.  (The lanes have read the stage's last block: the __syncwarp before.)
+    int st_in = 0, st_out = 0;                    // stages of the next block requested and taken
+    // Requests block `it` of the span.  A page that is not there is read as page 0 and masked later.  (The lanes have read
+    // the stage's last block: the __syncwarp before.)
     auto request = [&](int it) {
-        if (it >= n_iter) return;
-        const int st = n_in % kStages;
-        int page[SUB];
-#pragma unroll
-        for (int j = 0; j < SUB; ++j) page[j] = __shfl_sync(0xffffffffu, my_page, (it * SUB + j) & 31);
-        if (lane == 0) {
-            const uint32_t dst = ring_addr + st * C::kStage, bar = bar0 + 8 * st;
+        if (it < n_iter) {
+            const uint32_t dst = ring_addr + st_in * C::kStage + 16 * lane;
             const int key = s0 + (it * kSplitWarps + warp) * KB;
-            uint32_t bytes = 0;
-#pragma unroll
-            for (int j = 0; j < SUB; ++j) bytes += page[j] >= 0 ? 16 * (2 * D + 8) : 0;
-            tc::mbar_expect_tx(bar, bytes);
 #pragma unroll
             for (int j = 0; j < SUB; ++j) {
-                if (page[j] < 0) continue;
-                const size_t row = paged_row(a.p, page[j], h) + ((key + 16 * j) & ((1 << a.p.page_shift) - 1));
-                bulk_load(dst + 16 * j * D, a.p.k + row * D, 16 * D, bar);
-                bulk_load(dst + C::kOffV + 16 * j * D, a.p.v + row * D, 16 * D, bar);
-                bulk_load(dst + C::kOffKs + 64 * j, a.p.ks + row, 64, bar);
-                bulk_load(dst + C::kOffVs + 64 * j, a.p.vs + row, 64, bar);
+                const int page = max(__shfl_sync(0xffffffffu, my_page, (it * SUB + j) & 31), 0);
+                const size_t row = paged_row(a.p, page, h) + ((key + 16 * j) & ((1 << a.p.page_shift) - 1));
+                const int8_t *k = a.p.k + row * D + 16 * lane, *v = a.p.v + row * D + 16 * lane;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    cp_async16(dst + 16 * j * D + 512 * i, k + 512 * i);
+                    cp_async16(dst + C::kOffV + 16 * j * D + 512 * i, v + 512 * i);
+                }
+                if (lane < 8)                     // 64 bytes of each kind of scale
+                    cp_async16(dst + (lane < 4 ? C::kOffKs : C::kOffVs - 64) + 64 * j, (lane < 4 ? a.p.ks : a.p.vs - 16) + row + 4 * lane);
             }
+            st_in = st_in + 1 == kStages ? 0 : st_in + 1;
         }
-        ++n_in;
+        cp_async_commit();
     };
-    __syncwarp();
 #pragma unroll 1
     for (int i = 0; i < kStages; ++i) request(i);
 
@@ -239,16 +217,21 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
             for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
     }
 
-    int n_out = 0;                                // blocks taken so far
-    bool ok = true;
     for (;;) {
-    for (int it = 0; it < n_iter; ++it, ++n_out) {
+    for (int it = 0; it < n_iter; ++it) {
         const int k0 = s0 + (it * kSplitWarps + warp) * KB;
-        const unsigned char* blk = ring + (n_out % kStages) * C::kStage;
-        ok = wait_block(bar0 + 8 * (n_out % kStages), (n_out / kStages) & 1) && ok;
+        const unsigned char* blk = ring + st_out * C::kStage;
+        st_out = st_out + 1 == kStages ? 0 : st_out + 1;
+        cp_async_wait<kStages - 1>();
+        __syncwarp();                            // every lane's part of the block is there
+        // each value scale's logarithm and reciprocal once, not by all eight threads that need them
+        if (KB == 32 || lane < KB) {
+            const float v = fmaxf(reinterpret_cast<const float*>(blk + C::kOffVs)[lane], kLeastScale);
+            scaled[lane] = __log2f(v);
+            scaled[KB + lane] = __fdividef(1.0f, v);
+        }
+        __syncwarp();
         float sc[KG][4];
-        float2 inv[KG];
-        bool whole = true;                       // every key of the block is there
 #pragma unroll
         for (int u = 0; u < KG; ++u) {
 #pragma unroll
@@ -260,16 +243,12 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mma_f16(sc[u], qa[4 * i + e], bytes_to_half2(w[e], 0x4140), bytes_to_half2(w[e], 0x4342));
             }
-            const float2 ksr = *reinterpret_cast<const float2*>(blk + C::kOffKs + 32 * u + 8 * t), vsr = *reinterpret_cast<const float2*>(blk + C::kOffVs + 32 * u + 8 * t);
-            const float v0 = fmaxf(vsr.x, kLeastScale), v1 = fmaxf(vsr.y, kLeastScale);
-            const float b0 = __log2f(v0), b1 = __log2f(v1);
-            inv[u] = make_float2(__fdividef(1.0f, v0), __fdividef(1.0f, v1));
+            const float2 ksr = *reinterpret_cast<const float2*>(blk + C::kOffKs + 32 * u + 8 * t), lv = *reinterpret_cast<const float2*>(scaled + 8 * u + 2 * t);
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                sc[u][2 * n] = fmaf(sc[u][2 * n], alpha[n] * ksr.x, b0);
-                sc[u][2 * n + 1] = fmaf(sc[u][2 * n + 1], alpha[n] * ksr.y, b1);
+                sc[u][2 * n] = fmaf(sc[u][2 * n], alpha[n] * ksr.x, lv.x);
+                sc[u][2 * n + 1] = fmaf(sc[u][2 * n + 1], alpha[n] * ksr.y, lv.y);
             }
-            whole = whole && __shfl_sync(0xffffffffu, my_page, (it * SUB + (u >> 1)) & 31) >= 0;
         }
         if (!whole || shun || k0 + KB > c1 || (a.causal && k0 + KB - 1 > first)) {
 #pragma unroll
@@ -314,9 +293,10 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
             const float ref = m[n] == -INFINITY ? 0.0f : m[n];
 #pragma unroll
             for (int u = 0; u < KG; ++u) {
+                const float2 inv = *reinterpret_cast<const float2*>(scaled + KB + 8 * u + 2 * t);
                 const float p0 = exp2_fast(sc[u][2 * n] - ref), p1 = exp2_fast(sc[u][2 * n + 1] - ref);
-                l[n] = fmaf(p0, inv[u].x, l[n]);
-                l[n] = fmaf(p1, inv[u].y, l[n]);
+                l[n] = fmaf(p0, inv.x, l[n]);
+                l[n] = fmaf(p1, inv.y, l[n]);
                 const __half2 w = __floats2half2_rn(p0, p1);
                 pb[n][u] = *reinterpret_cast<const uint32_t*>(&w);
             }
@@ -358,7 +338,7 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
 #pragma unroll 1
     for (int i = 0; i < kStages; ++i) request(i);
     }
-    if (!ok && lane == 0) atomicCAS(a.p.status, 0, 0x40000000);
+    cp_async_wait<0>();
     __syncthreads();                             // no block is on its way any more: the rings' space is free
 
     // join the warps: statistics of row 8 n + g, then the outputs scaled to the CTA's maximum
@@ -418,22 +398,42 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
     if (!s_last) return;
     __threadfence();
     if (tid == 0) a.counters[unit] = 0;          // as the next launch expects it
-    for (int i = tid; i < n_rows * (D / 2); i += kSplitThreads) {
-        const int r = i / (D / 2), d = 2 * (i % (D / 2));
+    // A warp per row; the statistics of 32 chunks at a time, a lane each, then the chunks' outputs, several loads in flight.
+    for (int r = warp; r < n_rows; r += kSplitWarps) {
         const float* rec = part + (size_t)r * (D + 2);
-        float top = -INFINITY, sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
-        for (int sp = 0; sp < n_splits; ++sp) top = fmaxf(top, __ldcg(rec + (size_t)sp * ROWS * (D + 2)));
-        for (int sp = 0; sp < n_splits; ++sp) {
-            const float2 st = __ldcg(reinterpret_cast<const float2*>(rec + (size_t)sp * ROWS * (D + 2)));
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(rec + (size_t)sp * ROWS * (D + 2) + 2 + d));
-            if (st.x == -INFINITY) continue;
-            const float f = exp2_fast(st.x - top);
-            sum = fmaf(st.y, f, sum);
-            x0 = fmaf(v.x, f, x0);
-            x1 = fmaf(v.y, f, x1);
+        constexpr size_t kNext = (size_t)ROWS * (D + 2);
+        float top = -INFINITY;
+        for (int sp = lane; sp < n_splits; sp += 32) top = fmaxf(top, __ldcg(rec + sp * kNext));
+        top = warp_max(top);
+        float sum = 0.0f;
+        float2 x[D / 64];
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) x[i] = make_float2(0.0f, 0.0f);
+        for (int base = 0; base < n_splits; base += 32) {
+            float f = 0.0f;
+            if (base + lane < n_splits) {
+                const float2 st = __ldcg(reinterpret_cast<const float2*>(rec + (base + lane) * kNext));
+                f = st.x == -INFINITY ? 0.0f : exp2_fast(st.x - top);
+                sum = fmaf(st.y, f, sum);
+            }
+            const int n = min(32, n_splits - base);
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) {
+                const float2* v = reinterpret_cast<const float2*>(rec + (base + j) * kNext + 2) + lane;
+                const float fj = __shfl_sync(0xffffffffu, f, j);
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) {
+                    const float2 y = __ldcg(v + 32 * i);
+                    x[i].x = fmaf(y.x, fj, x[i].x);
+                    x[i].y = fmaf(y.y, fj, x[i].y);
+                }
+            }
         }
+        sum = warp_sum(sum);
         const float n = top == -INFINITY ? 0.0f : 1.0f / sum;
-        store_out<D>(a, s.q0 + (r0 + r) / a.G, h * a.G + (r0 + r) % a.G, d, x0 * n, x1 * n);
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i)
+            store_out<D>(a, s.q0 + (r0 + r) / a.G, h * a.G + (r0 + r) % a.G, 64 * i + 2 * lane, x[i].x * n, x[i].y * n);
     }
 }
 

@@ -44,12 +44,6 @@ constexpr float kLeastFactor = 1e-37f;
 constexpr float kNoReference = -1e30f;       // reference of a row that has seen no key: any visible key lies above it
 constexpr int kJoinRows = 32;                // rows a CTA of the join takes
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // One poll of a barrier, asleep for up to 20 us; a waiting warp that polls by itself takes issue slots from the working ones.
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
