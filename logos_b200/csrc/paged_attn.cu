@@ -13,7 +13,7 @@
 // fragments come straight from global memory: S = q K^T has the rows as M and the keys as N, O^T = V^T p has the
 // channels as M and the rows as N, and the accumulator of the first is the B operand of the second as it is, so p
 // never moves between threads.  The order of the channels inside a product is free, so a thread's share of a K row is
-// 16 consecutive bytes and its share of a V row DH / 8.  Blocks of 2 KiB of K and 2 KiB of V and their scales come by
+// 16 consecutive bytes and its share of a V row DH / 8.  Blocks of 32 keys and their scales come by
 // cp.async into a ring of each warp's own, kStages blocks in flight and no registers spent on them.  (By cp.async.bulk, one
 // lane for all, it took 80 instructions more a block, for the operands of its eight copies: 237 us where this takes 197, 64 sequences x
 // 16 heads x 8192 tokens.)  (tcgen05 needs 128 rows to be busy and its operands in shared memory; here a head has 1 to 16.)
@@ -68,8 +68,8 @@ __device__ __forceinline__ void store_out(const SplitArgs& a, int token, int hea
 
 // shared memory of a CTA: the warps' rings; the join of the warps uses their space
 template <int D, int NQ> struct SplitShape {
-    static constexpr int kRows = 8 * NQ, kKB = 2048 / D;      // keys of a block
-    static constexpr int kOffV = 2048, kOffKs = 4096, kOffVs = kOffKs + 4 * kKB, kStage = kOffVs + 4 * kKB;
+    static constexpr int kRows = 8 * NQ, kKB = 32;            // keys of a block
+    static constexpr int kOffV = kKB * D, kOffKs = 2 * kKB * D, kOffVs = kOffKs + 4 * kKB, kStage = kOffVs + 4 * kKB;
     static constexpr int kScaled = 8 * kKB;                   // log2 vs and 1 / vs of the warp's current block
     static constexpr int kRings = kSplitWarps * (kStages * kStage + kScaled);
     static constexpr int kPitch = D + 4;
@@ -225,7 +225,7 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
         cp_async_wait<kStages - 1>();
         __syncwarp();                            // every lane's part of the block is there
         // each value scale's logarithm and reciprocal once, not by all eight threads that need them
-        if (KB == 32 || lane < KB) {
+        {
             const float v = fmaxf(reinterpret_cast<const float*>(blk + C::kOffVs)[lane], kLeastScale);
             scaled[lane] = __log2f(v);
             scaled[KB + lane] = __fdividef(1.0f, v);
@@ -417,7 +417,7 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
                 sum = fmaf(st.y, f, sum);
             }
             const int n = min(32, n_splits - base);
-#pragma unroll 8
+#pragma unroll 16
             for (int j = 0; j < n; ++j) {
                 const float2* v = reinterpret_cast<const float2*>(rec + (base + j) * kNext + 2) + lane;
                 const float fj = __shfl_sync(0xffffffffu, f, j);

@@ -303,10 +303,10 @@ int qk_norm_rope(logos_ctx* ctx, int dtype, bool bwd, const void* Q, const void*
     for (int k = 0; k < rope->dims / 2; ++k) {
         const double f = rope->inv_freq[k];
         if (!std::isfinite(f)) return fail(ctx, LOGOS_ERR_INVALID_ARG, "%s: inv_freq[%d] is not finite", what, k);
-        const long double turns = (long double)f * 0.159154943091895335768883763372514362L;   // 1 / (2 pi)
-        const long double frac = turns - floorl(turns);
-        const long double scaled = ldexpl(frac, 64);
-        a.turns[k] = scaled >= 18446744073709551615.0L ? 0ull : (unsigned long long)scaled;
+        // (a frequency's 53 bits leave 2^31 positions 2^-22 of a turn: below fp32's own error of the angle)
+        const double turns = f * 0.15915494309189535;               // 1 / (2 pi)
+        const double frac = turns - std::floor(turns);
+        a.turns[k] = frac < 1.0 ? (unsigned long long)(frac * 0x1p64) : 0ull;
     }
     if (bwd && ((wq == nullptr) != (dwq == nullptr) || (wk == nullptr) != (dwk == nullptr)))
         return fail(ctx, LOGOS_ERR_INVALID_ARG, "%s: a weight and its gradient are given together", what);

@@ -20,6 +20,20 @@ def _ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)
 
 
+_STRIDES: dict = {}
+
+
+def _strides(row, head):
+    """Address of a logos_row_strides with these values."""
+    got = _STRIDES.get((row, head))
+    if got is None:
+        if len(_STRIDES) >= 4096:
+            _STRIDES.clear()
+        desc = L.RowStrides(row, head)
+        got = _STRIDES[(row, head)] = (C.addressof(desc), desc)
+    return got[0]
+
+
 class Engine:
     """One context per process and GPU (logos_ctx)."""
 
@@ -235,126 +249,153 @@ class Engine:
         return scales
 
     # ---- norm and rotation of queries and keys -----------------------------------
-    def _rows3(self, what, *tensors):
-        """Strides of [rows, H, DH] views (None stays None); the last dimension contiguous, one dtype, this device."""
-        first = next((t for t in tensors if t is not None), None)
-        if first is None:
-            raise ValueError(f"{what}: no tensor")
-        out = []
-        for t in tensors:
-            if t is None:
-                out.append(None)
-                continue
-            if t.dim() != 3 or (t.stride(2) != 1 and t.numel()):
-                raise ValueError(f"{what}: [rows, heads, DH] with contiguous channels, got {tuple(t.shape)} with strides {t.stride()}")
-            if t.dtype != first.dtype or t.shape[0] != first.shape[0] or t.shape[2] != first.shape[2]:
-                raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)} beside {first.dtype} {tuple(first.shape)}")
-            self._on_device(what, t)
-            out.append(C.byref(L.RowStrides(t.stride(0), t.stride(1))))
-        if first.dtype not in _DT:
-            raise ValueError(f"{what}: dtype {first.dtype}")
-        return out
+    # A serving loop makes these calls once per layer and token, so the checks are few and cheap, pointers travel as
+    # plain integers and the descriptors were laid out when their handles were made.
+    def _view(self, what, t, rows, heads, dh, dtype):
+        """Address of the strides of `t`, a [rows, heads, DH] view with contiguous channels on this device."""
+        if t.shape != (rows, heads, dh) or t.dtype != dtype:
+            raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)} where {dtype} {(rows, heads, dh)} is needed")
+        row, head, one = t.stride()
+        if one != 1 and t.numel():
+            raise ValueError(f"{what}: the channels of a row are contiguous, got strides {t.stride()}")
+        if t.get_device() != self.device:
+            raise ValueError(f"{what}: a tensor on {t.device}, the engine is on cuda:{self.device}")
+        return _strides(row, head)
 
-    def _on_device(self, what, *tensors):
-        for t in tensors:
-            if t is not None and (not t.is_cuda or t.device.index != self.device):
-                raise ValueError(f"{what}: a tensor on {t.device}, the engine is on cuda:{self.device}")
-
-    def _rope_args(self, what, Q, K, wq, wk, positions, rope):
-        rows, DH = (Q if Q is not None else K).shape[0::2]
-        for w in (wq, wk):
-            if w is not None and (w.dtype != torch.float32 or w.shape != (DH,) or not w.is_contiguous()):
-                raise ValueError(f"{what}: a weight is fp32 [{DH}], got {w.dtype} {tuple(w.shape)}")
-        if positions.dtype != torch.int32 or positions.shape != (rows,) or not positions.is_contiguous():
-            raise ValueError(f"{what}: positions are int32 [{rows}], got {positions.dtype} {tuple(positions.shape)}")
-        self._on_device(what, wq, wk, positions)
-        return rows, DH
+    def _rope_args(self, what, Q, K, wq, wk, positions):
+        first = Q if Q is not None else K
+        if first is None or first.dim() != 3 or first.dtype not in _DT:
+            raise ValueError(f"{what}: Q or K of [rows, heads, DH] in fp32, BF16 or FP16 is needed")
+        rows, _, DH = first.shape
+        for x, w in ((Q, wq), (K, wk)):
+            if w is not None and (x is None or w.dtype != torch.float32 or w.shape != (DH,) or not w.is_contiguous() or
+                                  w.get_device() != self.device):
+                raise ValueError(f"{what}: a weight is fp32 [{DH}] on cuda:{self.device} beside its tensor")
+        if (positions.dtype != torch.int32 or positions.shape != (rows,) or not positions.is_contiguous() or
+                positions.get_device() != self.device):
+            raise ValueError(f"{what}: positions are int32 [{rows}] on cuda:{self.device}, got {positions.dtype} "
+                             f"{tuple(positions.shape)} on {positions.device}")
+        return rows, DH, first.dtype
 
     def qk_norm_rope(self, Q, K, q_weight, k_weight, positions, rope, eps=1e-6, out_q=None, out_k=None):
         """Every head of Q [rows, Hq, DH] and K [rows, Hk, DH] (views with any row and head strides; either may be None)
         normalised by its RMS, weighted and rotated by its token's position, one kernel; a weight of None leaves that
-        norm out.  out_q / out_k: outputs (the inputs themselves for in place); None allocates packed ones."""
-        si = self._rows3("qk_norm_rope", Q, K)
-        rows, DH = self._rope_args("qk_norm_rope", Q, K, q_weight, k_weight, positions, rope)
-        out_q = torch.empty(Q.shape, dtype=Q.dtype, device=Q.device) if Q is not None and out_q is None else out_q
-        out_k = torch.empty(K.shape, dtype=K.dtype, device=K.device) if K is not None and out_k is None else out_k
-        so = self._rows3("qk_norm_rope", out_q, out_k)
-        for x, y in ((Q, out_q), (K, out_k)):
-            if (x is None) != (y is None) or (x is not None and (x.shape != y.shape or x.dtype != y.dtype)):
-                raise ValueError("qk_norm_rope: an output does not match its input")
-        self._check(self.lib.logos_qk_norm_rope(
-            self.h, _DT[(Q if Q is not None else K).dtype], _ptr(Q), _ptr(K), _ptr(q_weight), _ptr(k_weight), _ptr(positions),
-            C.byref(rope.desc), float(eps), _ptr(out_q), _ptr(out_k), rows, Q.shape[1] if Q is not None else 0,
-            K.shape[1] if K is not None else 0, DH, si[0], si[1], so[0], so[1]))
+        norm out.  out_q / out_k: outputs (the inputs themselves for in place); None allocates them, laid
+        out as the inputs are."""
+        what = "qk_norm_rope"
+        rows, DH, dtype = self._rope_args(what, Q, K, q_weight, k_weight, positions)
+        hq = hk = 0
+        q = k = yq = yk = sq = sk = syq = syk = None
+        if Q is not None:
+            hq = Q.shape[1]
+            sq = self._view(what, Q, rows, hq, DH, dtype)
+            if out_q is None:
+                out_q = torch.empty_like(Q)
+            syq = self._view(what, out_q, rows, hq, DH, dtype)
+            q, yq = Q.data_ptr(), out_q.data_ptr()
+        elif out_q is not None:
+            raise ValueError(f"{what}: an output without its input")
+        if K is not None:
+            hk = K.shape[1]
+            sk = self._view(what, K, rows, hk, DH, dtype)
+            if out_k is None:
+                out_k = torch.empty_like(K)
+            syk = self._view(what, out_k, rows, hk, DH, dtype)
+            k, yk = K.data_ptr(), out_k.data_ptr()
+        elif out_k is not None:
+            raise ValueError(f"{what}: an output without its input")
+        rc = self.lib.logos_qk_norm_rope(self.h, _DT[dtype], q, k, None if q_weight is None else q_weight.data_ptr(),
+                                         None if k_weight is None else k_weight.data_ptr(), positions.data_ptr(), rope.address,
+                                         eps, yq, yk, rows, hq, hk, DH, sq, sk, syq, syk)
+        if rc:
+            self._check(rc)
         return out_q, out_k
 
     def qk_norm_rope_bwd(self, Q, K, dQ_out, dK_out, q_weight, k_weight, positions, rope, eps=1e-6):
         """Gradients (dQ, dK, dq_weight, dk_weight) of qk_norm_rope for the gradients of its outputs; dQ and dK packed in
         the inputs' type, the weights' in fp32 (None where the weight, or the tensor, is None)."""
-        s = self._rows3("qk_norm_rope_bwd", Q, K, dQ_out, dK_out)
-        rows, DH = self._rope_args("qk_norm_rope_bwd", Q, K, q_weight, k_weight, positions, rope)
-        dx = []
-        for x, g, w in ((Q, dQ_out, q_weight), (K, dK_out, k_weight)):
-            if (x is None) != (g is None) or (x is not None and x.shape != g.shape) or (x is None and w is not None):
-                raise ValueError("qk_norm_rope_bwd: a gradient does not match its tensor")
-            dx.append(torch.empty(x.shape, dtype=x.dtype, device=x.device) if x is not None else None)
-        dwq, dwk = (torch.empty_like(w) if w is not None else None for w in (q_weight, k_weight))
-        args = (self.h, _DT[(Q if Q is not None else K).dtype], _ptr(Q), _ptr(K), _ptr(dQ_out), _ptr(dK_out), _ptr(q_weight),
-                _ptr(k_weight), _ptr(positions), C.byref(rope.desc), float(eps), _ptr(dx[0]), _ptr(dx[1]), _ptr(dwq), _ptr(dwk),
-                rows, Q.shape[1] if Q is not None else 0, K.shape[1] if K is not None else 0, DH, s[0], s[1], s[2], s[3],
-                None, None)
-        self._with_workspace(lambda: self.lib.logos_qk_norm_rope_bwd(*args),
-                             lambda: self.lib.logos_qk_norm_rope_bwd_workspace_bytes(DH))
-        return dx[0], dx[1], dwq, dwk
-
-    def _with_workspace(self, call, need):
-        """A call that reports a small workspace gets it reserved and runs again: no size query in the hot path."""
-        rc = call()
+        what = "qk_norm_rope_bwd"
+        rows, DH, dtype = self._rope_args(what, Q, K, q_weight, k_weight, positions)
+        if (Q is None) != (dQ_out is None) or (K is None) != (dK_out is None):
+            raise ValueError(f"{what}: a gradient without its tensor, or a tensor without its gradient")
+        hq = hk = 0
+        q = k = gq = gk = sq = sk = sgq = sgk = dQ = dK = dwq = dwk = None
+        if Q is not None:
+            hq = Q.shape[1]
+            sq, sgq = self._view(what, Q, rows, hq, DH, dtype), self._view(what, dQ_out, rows, hq, DH, dtype)
+            q, gq, dQ = Q.data_ptr(), dQ_out.data_ptr(), torch.empty((rows, hq, DH), dtype=dtype, device=Q.device)
+        if K is not None:
+            hk = K.shape[1]
+            sk, sgk = self._view(what, K, rows, hk, DH, dtype), self._view(what, dK_out, rows, hk, DH, dtype)
+            k, gk, dK = K.data_ptr(), dK_out.data_ptr(), torch.empty((rows, hk, DH), dtype=dtype, device=K.device)
+        if q_weight is not None:
+            dwq = torch.empty_like(q_weight)
+        if k_weight is not None:
+            dwk = torch.empty_like(k_weight)
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        args = (self.h, _DT[dtype], q, k, gq, gk, ptr(q_weight), ptr(k_weight), positions.data_ptr(), rope.address, eps, ptr(dQ),
+                ptr(dK), ptr(dwq), ptr(dwk), rows, hq, hk, DH, sq, sk, sgq, sgk, None, None)
+        rc = self.lib.logos_qk_norm_rope_bwd(*args)
         if rc == L.ERR_WORKSPACE:
-            self.reserve(need())
-            rc = call()
-        self._check(rc)
+            self.reserve(self.lib.logos_qk_norm_rope_bwd_workspace_bytes(DH))
+            rc = self.lib.logos_qk_norm_rope_bwd(*args)
+        if rc:
+            self._check(rc)
+        return dQ, dK, dwq, dwk
 
     # ---- paged INT8 KV ---------------------------------------------------------
+    def _paged(self, what, cache, batch, rows):
+        if cache.device_index != self.device or batch.device_index != self.device:
+            raise ValueError(f"{what}: cache on device {cache.device_index}, batch on {batch.device_index}, the engine on {self.device}")
+        batch.desc.rows = rows
+
     def paged_append(self, K, V, cache, batch):
         """The batch's new K and V rows ([rows, H, DH], any row and head strides) quantised into their pages, a scale
         per row.  rows may exceed the batch's last row: those are not read."""
-        s = self._rows3("paged_append", K, V)
-        self._paged_args("paged_append", K, V, cache, batch)
-        self._check(self.lib.logos_paged_append(self.h, _DT[K.dtype], _ptr(K), _ptr(V), s[0], s[1], C.byref(cache.desc),
-                                                C.byref(batch.desc)))
+        what, rows, dtype = "paged_append", K.shape[0], K.dtype
+        sk = self._view(what, K, rows, cache.heads, cache.dh, dtype)
+        sv = self._view(what, V, rows, cache.heads, cache.dh, dtype)
+        self._paged(what, cache, batch, rows)
+        rc = self.lib.logos_paged_append(self.h, _DT.get(dtype, -1), K.data_ptr(), V.data_ptr(), sk, sv, cache.address, batch.address)
+        if rc:
+            self._check(rc)
 
     def paged_read(self, cache, batch, out_k, out_v):
         """The values the cache holds for the batch's rows -> out_k, out_v ([rows, H, DH], fp32 or 16-bit, any row and
         head strides); rows behind the last sequence stay as they are."""
-        s = self._rows3("paged_read", out_k, out_v)
-        self._paged_args("paged_read", out_k, out_v, cache, batch)
-        self._check(self.lib.logos_paged_read(self.h, _DT[out_k.dtype], C.byref(cache.desc), C.byref(batch.desc), _ptr(out_k),
-                                              _ptr(out_v), s[0], s[1]))
+        what, rows, dtype = "paged_read", out_k.shape[0], out_k.dtype
+        sk = self._view(what, out_k, rows, cache.heads, cache.dh, dtype)
+        sv = self._view(what, out_v, rows, cache.heads, cache.dh, dtype)
+        self._paged(what, cache, batch, rows)
+        rc = self.lib.logos_paged_read(self.h, _DT.get(dtype, -1), cache.address, batch.address, out_k.data_ptr(), out_v.data_ptr(), sk, sv)
+        if rc:
+            self._check(rc)
         return out_k, out_v
-
-    def _paged_args(self, what, K, V, cache, batch):
-        if K.shape != V.shape or K.shape[1:] != (cache.heads, cache.dh):
-            raise ValueError(f"{what}: K {tuple(K.shape)}, V {tuple(V.shape)} for a cache of {cache.heads} heads of {cache.dh}")
-        self._on_device(what, cache.k, batch.cu_q)
-        batch.desc.rows = K.shape[0]
 
     def paged_attention(self, Q, cache, batch, params: L.Params, out=None):
         """Attention of the batch's new tokens Q [rows, Hq, DH] (BF16 or FP16, any row and head strides) over the pages
         -> [rows, Hq, DH].  Append their K and V first.  With `out`, rows behind the last sequence stay as they are;
-        without it they are undefined."""
+        without it they are undefined.  Before capturing a graph, run the call once or reserve its workspace
+        (paged_attention_workspace_bytes)."""
+        what, dtype = "paged_attention", Q.dtype
+        rows, Hq, DH = Q.shape
         if out is None:
-            out = torch.empty(Q.shape, dtype=Q.dtype, device=Q.device)
-        s = self._rows3("paged_attention", Q, out)
-        if out.shape != Q.shape or Q.shape[2] != cache.dh:
-            raise ValueError(f"paged_attention: Q {tuple(Q.shape)}, out {tuple(out.shape)}, heads of {cache.dh} in the cache")
-        self._on_device("paged_attention", cache.k, batch.cu_q)
-        batch.desc.rows, Hq = Q.shape[0], Q.shape[1]
-        self._with_workspace(
-            lambda: self.lib.logos_paged_attention(self.h, _DT[Q.dtype], _ptr(Q), C.byref(cache.desc), C.byref(batch.desc), Hq,
-                                                   C.byref(params), _ptr(out), s[0], s[1]),
-            lambda: self.lib.logos_paged_attention_workspace_bytes(self.h, C.byref(cache.desc), C.byref(batch.desc), Hq))
+            out = torch.empty((rows, Hq, DH), dtype=dtype, device=Q.device)
+        sq = self._view(what, Q, rows, Hq, cache.dh, dtype)
+        so = self._view(what, out, rows, Hq, DH, dtype)
+        self._paged(what, cache, batch, rows)
+        args = (self.h, _DT.get(dtype, -1), Q.data_ptr(), cache.address, batch.address, Hq, C.byref(params), out.data_ptr(), sq, so)
+        rc = self.lib.logos_paged_attention(*args)
+        if rc == L.ERR_WORKSPACE:
+            self.reserve(self.paged_attention_workspace_bytes(cache, batch, rows, Hq))
+            rc = self.lib.logos_paged_attention(*args)
+        if rc:
+            self._check(rc)
         return out
+
+    def paged_attention_workspace_bytes(self, cache, batch, rows, Hq):
+        self._paged("paged_attention", cache, batch, rows)
+        return self.lib.logos_paged_attention_workspace_bytes(self.h, cache.address, batch.address, Hq)
 
     # ---- Nikhilam INT8 KV ----------------------------------------------------
     def prefill(self, Q, K, V, params: L.Params, k_cache, v_cache, k_scale, v_scale, out_dtype=None, out=None):

@@ -102,15 +102,14 @@ SIGNATURES = {
     "logos_decode_int8_gather": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _PP, _vp]),
     "logos_decode_step_int8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _PP, _vp]),
     "logos_decode_step_int8_to": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _PP, _i, _vp]),
-    "logos_qk_norm_rope": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, C.POINTER(Rope), _f, _vp, _vp, _i, _i, _i, _i, _vp, _vp,
-                                _vp, _vp]),
+    "logos_qk_norm_rope": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "logos_qk_norm_rope_bwd_workspace_bytes": (_sz, [_i]),
-    "logos_qk_norm_rope_bwd": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.POINTER(Rope), _f, _vp, _vp, _vp, _vp, _i,
+    "logos_qk_norm_rope_bwd": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _vp, _vp, _vp, _i,
                                     _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "logos_paged_append": (_i, [_vp, _i, _vp, _vp, _vp, _vp, C.POINTER(PagedCache), C.POINTER(PagedBatch)]),
-    "logos_paged_read": (_i, [_vp, _i, C.POINTER(PagedCache), C.POINTER(PagedBatch), _vp, _vp, _vp, _vp]),
-    "logos_paged_attention_workspace_bytes": (_sz, [_vp, C.POINTER(PagedCache), C.POINTER(PagedBatch), _i]),
-    "logos_paged_attention": (_i, [_vp, _i, _vp, C.POINTER(PagedCache), C.POINTER(PagedBatch), _i, _PP, _vp, _vp, _vp]),
+    "logos_paged_append": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "logos_paged_read": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "logos_paged_attention_workspace_bytes": (_sz, [_vp, _vp, _vp, _i]),
+    "logos_paged_attention": (_i, [_vp, _i, _vp, _vp, _vp, _i, _PP, _vp, _vp, _vp]),
     "logos_layer_norm": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, C.c_float]),
     "logos_decode_step_int8_gather": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i,
                                           _PP, _vp]),

@@ -31,6 +31,7 @@ class Rope:
             raise ValueError(f"Rope: {len(f)} frequencies for {dims // 2} pairs")
         self.dims, self.interleaved, self.inv_freq = dims, bool(interleaved), tuple(f)
         self.desc = L.Rope(dims, int(bool(interleaved)), (C.c_double * L.ROPE_MAX_PAIRS)(*f))
+        self.address = C.addressof(self.desc)
 
 
 def _need(t: torch.Tensor, dtype, what: str):
@@ -68,6 +69,7 @@ class PagedKVCache:
         self.pages, self.heads, self.page_size, self.dh = k.shape
         self.desc = L.PagedCache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), self.pages, self.page_size,
                                  self.heads, self.dh)
+        self.address, self.device_index = C.addressof(self.desc), k.get_device()
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.ks, self.vs))
@@ -97,6 +99,7 @@ class PagedBatch:
         self.B, self.max_q, self.max_kv = B, int(max_q), int(max_kv)
         self.desc = L.PagedBatch(cu_q.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), B, page_table.shape[1], 0,
                                  self.max_q, self.max_kv)
+        self.address, self.device_index = C.addressof(self.desc), cu_q.get_device()
 
     def positions(self, rows: int) -> torch.Tensor:
         """int32 [rows]: the position of every token row (0 for rows behind the last sequence)."""

@@ -97,6 +97,32 @@ def test_append_and_read(engine, n_q, n_kv, H, D, page, layout, dtype, pad):
             assert torch.equal(y[rows:], torch.full_like(y[rows:], 7.0))
 
 
+def test_append_rounds_as_the_division_does(engine):
+    """Values on the border between two bytes, a step to either side of it, and rows with an infinity or a NaN: the bytes of
+    the fp32 division, rounded half to even."""
+    g = torch.Generator().manual_seed(6)
+    rows, H, D = 512, 4, 64
+    top = 10.0 ** (torch.rand((rows, H, 1), generator=g) * 12 - 8)
+    scale = (top + torch.tensor(1e-8)) / torch.tensor(127.5)
+    half = torch.randint(-127, 127, (rows, H, D), generator=g).float() + 0.5
+    x = half * scale
+    up = torch.rand(x.shape, generator=g)
+    x = torch.where(up < 0.3, torch.nextafter(x, torch.tensor(float("inf"))), torch.where(up > 0.7, torch.nextafter(x, torch.tensor(0.0)), x))
+    x[..., :1] = top                                        # the row's largest value
+    x = torch.minimum(torch.maximum(x, -top), top)
+    x[3, 1, 5], x[4, 2, 6], x[5, 0, :] = float("inf"), float("nan"), 0.0
+    pages, batch = tables([rows], [rows], 64)
+    cache = fresh(pages, H, 64, D)
+    engine.paged_append(x.cuda(), x.cuda(), cache, batch)
+    where = rows_of(batch, 64)
+    at, off = (torch.tensor([w[i] for w in where], dtype=torch.long) for i in range(2))
+    # the kernel's maximum passes over a NaN, and a quotient that is none counts as 0
+    s = (x.abs().nan_to_num(nan=0.0, posinf=float("inf")).amax(-1) + torch.tensor(1e-8)) / torch.full((rows, H), 127.5)
+    q = torch.clamp(torch.round((x / s[..., None]).nan_to_num(nan=0.0)), -127, 127).to(torch.int8)
+    for c8, cs in ((cache.k, cache.ks), (cache.v, cache.vs)):
+        assert torch.equal(c8.cpu()[at, :, off], q) and torch.equal(cs.cpu()[at, :, off], s)
+
+
 def attend64(Q, cache, batch, params, page):
     """(output, sum w |v|, sum |v8| max vs) in 64 bits, row by row of the batch; zeros where nothing is seen."""
     cu, kv, table = batch.cu_q.tolist(), batch.kv_len.tolist(), batch.page_table
@@ -347,7 +373,7 @@ def test_captured_step_replays_with_new_lengths(engine):
     eng.use_stream(stream)
     buf = [torch.empty((3, H, D), dtype=torch.bfloat16, device="cuda") for _ in range(4)]
     pos = torch.empty(3, dtype=torch.int32, device="cuda")
-    eng.reserve(eng.lib.logos_paged_attention_workspace_bytes(eng.h, cache.desc, _with_rows(batch.desc, 3), H))
+    eng.reserve(eng.paged_attention_workspace_bytes(cache, batch, 3, H))
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
         for t in buf:
@@ -367,11 +393,6 @@ def test_captured_step_replays_with_new_lengths(engine):
     eng.synchronize()
     del graph
     eng.close()
-
-
-def _with_rows(desc, rows):
-    desc.rows = rows
-    return desc
 
 
 def test_chunks_and_steps_give_what_one_pass_gives(engine):
@@ -443,6 +464,7 @@ def test_refusals(engine):
                 lambda: engine.paged_attention(Q.cpu(), cache, batch, params),
                 lambda: engine.paged_append(Q, Q[:, :1], cache, batch),
                 lambda: engine.paged_append(Q[:, :1], Q[:, :1], cache, batch),
+                lambda: engine.paged_append(Q.transpose(1, 2), Q, cache, batch),
                 lambda: engine.paged_read(cache, batch, Q, Q.half())):
         with pytest.raises(ValueError):
             bad()
