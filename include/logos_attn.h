@@ -505,8 +505,8 @@ int logos_paged_read(logos_ctx* ctx, int dtype, const logos_paged_cache* cache, 
  * than the window.  The Navier-Stokes terms are not offered here (LOGOS_ERR_UNSUPPORTED: apply the advection to
  * Q and the diffusion to V before they get here); scale > 0.  A row that sees nothing gets zeros.
  * The int8 values enter the products exactly, the scales stay fp32; weights are rounded to FP16 once, sums are fp32.
- * Results do not depend on what else is in the batch beyond the split of the keys, which the bounds decide;
- * the same call gives the same bits.  O may not overlap Q.  Workspace from the context
+ * The same call gives the same bits; another batch around a sequence may cut its keys at other places and so change
+ * the order of its sums.  O may not overlap Q.  Workspace from the context
  * (logos_paged_attention_workspace_bytes / logos_ctx_reserve); calls that share a context run one after the other. */
 size_t logos_paged_attention_workspace_bytes(logos_ctx* ctx, const logos_paged_cache* cache,
                                              const logos_paged_batch* batch, int Hq);

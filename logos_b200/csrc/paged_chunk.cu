@@ -40,6 +40,7 @@ constexpr int kRegsSoftmax = 88, kRegsConvert = 48, kRegsRest = 56;      // the 
 static_assert(512 * kRegsSoftmax + 256 * kRegsConvert + 128 * kRegsRest <= kChunkThreads * 72 && kChunkThreads * 72 <= 65536, "registers");
 constexpr int kScaleStages = 4, kSegStages = 4;
 constexpr int kSegReaders = kPlanWarp;       // warps 0 ... 25 read every segment
+constexpr int kItemCost = 4;                  // what an item costs beside its tiles (queries in, pipeline filled, rows out), in tiles
 constexpr float kLeastFactor = 1e-37f;
 constexpr float kNoReference = -1e30f;       // reference of a row that has seen no key: any visible key lies above it
 constexpr int kJoinRows = 32;                // rows a CTA of the join takes
@@ -153,12 +154,13 @@ __device__ __forceinline__ Item item_keys(const ChunkArgs& a, const PagedSeq& s,
     it.tiles = (it.end - it.begin + kBN - 1) / kBN;
     return it;
 }
-// key tiles of one head of a sequence; 0 when the sequence is not this kernel's
+// length of one head of a sequence on the line of work: its items' key tiles and kItemCost for each item; 0 when the
+// sequence is not this kernel's
 __device__ __forceinline__ long long seq_tiles(const ChunkArgs& a, int b) {
     const PagedSeq s = paged_seq(a.p, b);
     if (!s.ok || (long long)s.n * a.G <= a.min_rows) return 0;
     long long sum = 0;
-    for (int r = 0; r < s.n * a.G; r += kChunkRows) sum += item_keys(a, s, r, min(kChunkRows, s.n * a.G - r)).tiles;
+    for (int r = 0; r < s.n * a.G; r += kChunkRows) sum += item_keys(a, s, r, min(kChunkRows, s.n * a.G - r)).tiles + kItemCost;
     return sum;
 }
 
@@ -226,7 +228,7 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
         if (pass == 0) {
             total = run;
             share = (total + gridDim.x - 1) / gridDim.x;
-            if (share < 2) share = 2;                       // a shorter run costs more in joining than it saves
+            if (share < kItemCost + 2) share = kItemCost + 2;   // a shorter run costs more in joining than it saves
             my0 = (long long)blockIdx.x * share;
             my1 = my0 + share < total ? my0 + share : total;
             if (my0 >= total) break;
@@ -258,18 +260,24 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                     for (; ok && h < a.p.H && at < my1; ++h) {
                         for (int row0 = 0; ok && row0 < n_rows && at < my1; row0 += kChunkRows) {
                             const Item it = item_keys(a, s, row0, min(kChunkRows, n_rows - row0));
-                            if (off >= it.tiles) { off -= it.tiles; continue; }
+                            const int span = it.tiles + kItemCost;      // the item's stretch of the line: its cost, then its tiles
+                            if (off >= span) { off -= span; continue; }
+                            const long long left = my1 - at, rest = span - off;
+                            const long long take = rest < left ? rest : left;
+                            const int t0 = off > kItemCost ? (int)off - kItemCost : 0, t1 = (int)(off + take) - kItemCost;
+                            const long long item0 = at - off;
+                            at += take;
+                            off = 0;
+                            if (t1 <= t0) continue;                       // the share ends before the item's first tile
                             Segment g;
                             g.b = b; g.h = h; g.row0 = row0; g.n_rows = n_rows;
                             g.q0 = s.q0; g.n = s.n; g.kv = s.kv; g.begin = it.begin; g.end = it.end;
-                            g.i0 = (int)off;
-                            const long long left = my1 - at, rest = it.tiles - off;
-                            g.n_iter = (int)(rest < left ? rest : left);
-                            const bool whole = g.i0 == 0 && g.n_iter == it.tiles;
+                            g.i0 = t0;
+                            g.n_iter = t1 - t0;
+                            const bool whole = t0 == 0 && t1 == it.tiles;
                             g.slot = whole ? -1 : (int)blockIdx.x * 2 + (n_seg > 0 ? 1 : 0);
-                            if (g.i0 == 0 && !whole) {       // it goes on in the next CTAs: this one names it for the join
-                                const long long item0 = at;
-                                meta.parts = (int)((item0 + it.tiles - 1) / share - item0 / share) + 1;
+                            if (t0 == 0 && !whole) {         // it goes on in the next CTAs: this one names it for the join
+                                meta.parts = (int)((item0 + span - 1) / share - (item0 + kItemCost) / share) + 1;
                                 meta.slot = g.slot; meta.b = b; meta.h = h; meta.row0 = row0; meta.n_rows = n_rows; meta.q0 = s.q0;
                             }
                             const int st = n_seg % kSegStages;
@@ -277,8 +285,6 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                             *reinterpret_cast<Segment*>(smem + C::kOffSeg + st * 64) = g;
                             mbar_arrive(bar(SEGFULL + st));
                             ++n_seg;
-                            at += g.n_iter;
-                            off = 0;
                         }
                     }
                     base += per_head * a.p.H;
@@ -538,9 +544,11 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                 const volatile Segment* seg = reinterpret_cast<const volatile Segment*>(smem + C::kOffSeg + sst * 64);
                 if (seg->n_iter == 0) break;
                 int lo = 0, hi = 0;                   // tiles of the item that this row tile takes part in
+                bool rows_here = false;               // some of the warp's 16 rows are query rows
                 int e_hi = 0x7fffffff, e_lo = -0x7fffffff;   // a tile whose first key lies outside [e_lo, e_hi] is masked in part
                 {
                     const int n_rows = seg->n_rows, r0 = seg->row0 + 128 * g;
+                    rows_here = r0 + wr < n_rows;
                     if (r0 < n_rows) {
                         PagedSeq s; s.q0 = seg->q0; s.n = seg->n; s.kv = seg->kv; s.ok = true;
                         const int rows = min(128, n_rows - r0), begin = seg->begin;
@@ -587,6 +595,14 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                     const float* sa = reinterpret_cast<const float*>(smem + C::kOffScale + sc * C::kScaleBytes) + col;
                     if (!wait_w(bar(SFULL + g), s_run & 1)) { ok = false; break; }
                     tc_fence_after();
+                    if (!rows_here) {                 // rows behind the last one: what P holds for them reaches no output
+                        arrive_w(bar(SCEMPTY + sc));
+                        if (C::kOwnP) arrive_w(bar(SEMPTY + g));
+                        arrive_w(bar(PFULL + g));
+                        ++s_run;
+                        first = false;
+                        continue;
+                    }
                     if (k0 > e_hi || k0 < e_lo) {
                         // Some rows do not see some of the keys: -inf on their scores, in tensor memory, before the loop below.
                         // (Inside it the test and the code would cost every tile registers and instruction fetches.)

@@ -297,6 +297,10 @@ def test_bad_tables_are_reported_and_touch_nothing_else(engine):
             assert e.value.status == L.ERR_BAD_BATCH and "sequence 1" in str(e.value) and "page" in str(e.value)
             assert torch.equal(got[:n_q], clean[:n_q]) and torch.equal(got[2 * n_q:], clean[2 * n_q:])
         batch.page_table.copy_(keep)
+        # Without sequence 0 the work of the others may be cut at other keys, so their sums run in another order: either
+        # result is within check_attention's bound of the exact one, the two within twice that of each other.
+        want, size, tiny = attend64(Q, cache, batch, params, 64)
+        bound = 2 * ((2.0 ** -11 + 2.0 ** -13) * size + 2.0 ** -25 * tiny + torch.finfo(Q.dtype).eps / 2 * want.abs() + 1e-7)
         kv = batch.kv_len.clone()
         for value in (501, -1, n_q - 1):
             batch.kv_len[0] = value
@@ -305,7 +309,8 @@ def test_bad_tables_are_reported_and_touch_nothing_else(engine):
             with pytest.raises(L.LogosError) as e:
                 engine.synchronize()
             assert e.value.status == L.ERR_BAD_BATCH and "sequence 0" in str(e.value)
-            assert torch.equal(got[n_q:], clean[n_q:]) and torch.equal(got[:n_q], torch.full_like(got[:n_q], 5.0))
+            assert ((got.double() - clean.double()).abs() - bound)[n_q:].max().item() <= 0
+            assert torch.equal(got[:n_q], torch.full_like(got[:n_q], 5.0))
         batch.kv_len.copy_(kv)
         # append and read: a bad page leaves its rows alone
         before = cache.k.clone()
