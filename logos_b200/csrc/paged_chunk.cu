@@ -102,16 +102,17 @@ __device__ __forceinline__ void ld_scores(uint32_t taddr, float (&x)[kBW / 2]) {
 
 template <int D> struct Shape {
     static constexpr int kTile = kBN * D * 2;                 // one FP16 tile of 128 rows
-    static constexpr int kStages = D == 64 ? 3 : 2;
+    static constexpr int kStages = D == 64 ? 3 : 2;           // K tiles
+    static constexpr int kStagesV = D == 64 ? 3 : 2;          // V tiles
     static constexpr bool kOwnP = D == 64;                    // P has TMEM columns of its own
     static constexpr int kOffQ = 0, kOffK = kOffQ + 2 * kTile, kOffV = kOffK + kStages * kTile;
-    static constexpr int kOffScale = kOffV + kStages * kTile; // kScaleStages x {a, b, 1/vs: 128 floats each, 4 words of landmarks}
+    static constexpr int kOffScale = kOffV + kStagesV * kTile; // kScaleStages x {a, b, 1/vs: 128 floats each, 4 words of landmarks}
     static constexpr int kScaleBytes = 3 * kBN * 4 + 16;
     static constexpr int kDepth = D == 64 ? 4 : 3;            // pieces of 1 KiB a converting warp has in flight
     static constexpr int kOffRaw = kOffScale + kScaleStages * kScaleBytes;
     static constexpr int kOffSeg = kOffRaw + 8 * kDepth * 1024;
     static constexpr int kOffBar = kOffSeg + kSegStages * 64;
-    static constexpr int kNumBars = 4 * kStages + 2 * kScaleStages + 2 * kSegStages + 5 * 2 + 1;
+    static constexpr int kNumBars = 2 * (kStages + kStagesV) + 2 * kScaleStages + 2 * kSegStages + 5 * 2 + 1;
     static constexpr int kOffScan = kOffBar + kNumBars * 8;
     static constexpr int kSmem = kOffScan + 8 * (kChunkThreads / 32) + 1024;       // + alignment slack
     static constexpr int kColO = 256, kColP = 384;
@@ -168,8 +169,8 @@ template <int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
 paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
     using C = Shape<D>;
-    constexpr int ST = C::kStages;
-    enum Bar { KFULL = 0, KEMPTY = KFULL + ST, VFULL = KEMPTY + ST, VEMPTY = VFULL + ST, SCFULL = VEMPTY + ST,
+    constexpr int ST = C::kStages, SV = C::kStagesV;
+    enum Bar { KFULL = 0, KEMPTY = KFULL + ST, VFULL = KEMPTY + ST, VEMPTY = VFULL + SV, SCFULL = VEMPTY + SV,
                SCEMPTY = SCFULL + kScaleStages, SEGFULL = SCEMPTY + kScaleStages, SEGEMPTY = SEGFULL + kSegStages,
                SFULL = SEGEMPTY + kSegStages, SEMPTY = SFULL + 2, PFULL = SEMPTY + 2, PVDONE = PFULL + 2, QREADY = PVDONE + 2,
                DRAIN = QREADY + 2, NBARS };
@@ -187,7 +188,8 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int i = 0; i < ST; ++i) { mbar_init(bar(KFULL + i), 4); mbar_init(bar(KEMPTY + i), 2); mbar_init(bar(VFULL + i), 4); mbar_init(bar(VEMPTY + i), 2); }
+        for (int i = 0; i < ST; ++i) { mbar_init(bar(KFULL + i), 4); mbar_init(bar(KEMPTY + i), 2); }
+        for (int i = 0; i < SV; ++i) { mbar_init(bar(VFULL + i), 4); mbar_init(bar(VEMPTY + i), 2); }
         for (int i = 0; i < kScaleStages; ++i) { mbar_init(bar(SCFULL + i), 4); mbar_init(bar(SCEMPTY + i), 16); }
         for (int i = 0; i < kSegStages; ++i) { mbar_init(bar(SEGFULL + i), 1); mbar_init(bar(SEGEMPTY + i), kSegReaders); }
         for (int g = 0; g < 2; ++g) {
@@ -355,10 +357,10 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                     return true;
                 };
                 auto issue_pv = [&](int i, bool first) {
-                    const int st = nv % ST;
+                    const int st = nv % SV;
                     const bool on = i >= lo && i < hi;
                     if (on && !wait_w(bar(PFULL + g), s_pv & 1)) return false;
-                    if (!wait_w(bar(VFULL + st), (nv / ST) & 1)) return false;
+                    if (!wait_w(bar(VFULL + st), (nv / SV) & 1)) return false;
                     if (on) {
                         tc_fence_after();
                         const uint32_t vl = v_lo0 + (uint32_t)st * (C::kTile >> 4);
@@ -434,7 +436,7 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                     report_batch(a.p.status, sb, true);
                     return -1;
                 };
-                int pg = checked(entries_from(0)), pg_next = entries_from(16);
+                int pg = checked(entries_from(0)), pg_next = entries_from(16), pg_last = pg, group = 0;   // group: 16 tiles that pg is for
                 float ks = 0.0f, vs = 0.0f;                          // the scales of this thread's key of the tile
                 bool there = false;
                 int slot_in = 0, slot_out = 0;
@@ -443,7 +445,7 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                 auto fetch = [&](int n) {
                     if (n < PPT * n_iter) {
                         const int i = n / PPT, blk = n % PPT;
-                        if (n % (16 * PPT) == 0 && n > 0) { pg = checked(pg_next); pg_next = entries_from(i + 16); }
+                        if (n % (16 * PPT) == 0 && n > 0) { pg_last = pg; pg = checked(pg_next); pg_next = entries_from(i + 16); ++group; }
                         const int key = key_first + i * kBN + PR * blk;
                         const int page = max(__shfl_sync(0xffffffffu, pg, 2 * (i & 15) + (PR * blk >> 4)), 0);
                         const int8_t* at = src + (paged_row(a.p, page, sh) + (key & page_mask) + r16) * D + 16 * c16;
@@ -456,7 +458,9 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                 auto fetch_scales = [&](int i) {
                     if (is_v || i >= n_iter) return;
                     const int key = key_first + i * kBN + lane;
-                    const int page = __shfl_sync(0xffffffffu, (i & 15) == 0 && i > 0 ? pg_next : pg, 2 * (i & 15) + (lane >> 4));
+                    // (the fetches are up to kDepth - 1 pieces ahead of this tile, or just short of it)
+                    const int d = (i >> 4) - group;
+                    const int page = __shfl_sync(0xffffffffu, d > 0 ? pg_next : d < 0 ? pg_last : pg, 2 * (i & 15) + (lane >> 4));
                     there = (unsigned)page < (unsigned)a.p.pages && key < end;
                     const size_t row = paged_row(a.p, there ? page : 0, sh) + (key & page_mask);
                     ks = __ldg(a.p.ks + row);
@@ -483,8 +487,8 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                         arrive_w(bar(SCFULL + sc));
                         fetch_scales(i + 1);
                     }
-                    const int st = n_t % ST;
-                    if (n_t >= ST && !wait_w(bar(EMPTY + st), ((n_t / ST) - 1) & 1)) { ok = false; break; }
+                    const int depth = is_v ? SV : ST, st = n_t % depth;
+                    if (n_t >= depth && !wait_w(bar(EMPTY + st), ((n_t / depth) - 1) & 1)) { ok = false; break; }
                     unsigned char* tile = tiles + st * C::kTile + (c16 >> 2) * 16384 + (w32 + r16) * 128;
 #pragma unroll 1
                     for (int blk = 0; blk < PPT; ++blk) {
@@ -536,12 +540,34 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
             auto arrive_w = [&](uint32_t bb) { __syncwarp(); if (lane == 0) mbar_arrive(bb); };
             int n_t = 0, s_run = 0;                   // key tiles seen, score tiles of this row tile taken
             bool ok = true;
+            // The warp's query rows of segment n into shared memory as they are, half a row a thread.  The products of the segment
+            // before are all done when its last scores have come.
+            auto segment = [&](int n) { return reinterpret_cast<const volatile Segment*>(smem + C::kOffSeg + (n % kSegStages) * 64); };
+            auto load_q = [&](int n) {
+                if (!wait_w(bar(SEGFULL + n % kSegStages), (n / kSegStages) & 1)) return false;
+                const volatile Segment* seg = segment(n);
+                if (seg->n_iter == 0) return true;
+                const int r = wr + (lane >> 1), row0 = seg->row0, row = row0 + 128 * g + r;
+                const bool live = row < seg->n_rows;
+                const int token = (live ? row : row0) / a.G, head = seg->h * a.G + (live ? row : row0) % a.G;
+                const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(seg->q0 + token) * a.q_row + (long long)head * a.q_head;
+                unsigned char* dst = smem + C::kOffQ + g * C::kTile + r * 128;
+                constexpr int N = D / 16;
+                const int i0 = (lane & 1) * N;
+                uint4 w[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) w[i] = live ? *reinterpret_cast<const uint4*>(src + 8 * (i0 + i)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < N; ++i) *reinterpret_cast<uint4*>(dst + ((i0 + i) >> 3) * 16384 + ((((i0 + i) & 7) ^ (r & 7)) << 4)) = w[i];
+                fence_async_smem();
+                arrive_w(bar(QREADY + g));
+                return true;
+            };
+            ok = load_q(0);
             for (int n_seg = 0; ok; ++n_seg) {
-                const int sst = n_seg % kSegStages;
-                if (!wait_w(bar(SEGFULL + sst), (n_seg / kSegStages) & 1)) break;
                 // The segment stays where it is, and its slot this warp's, until its output is written: its fields are read when they
                 // are wanted and hold no registers meanwhile.
-                const volatile Segment* seg = reinterpret_cast<const volatile Segment*>(smem + C::kOffSeg + sst * 64);
+                const volatile Segment* seg = segment(n_seg);
                 if (seg->n_iter == 0) break;
                 int lo = 0, hi = 0;                   // tiles of the item that this row tile takes part in
                 bool rows_here = false;               // some of the warp's 16 rows are query rows
@@ -560,24 +586,6 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                         if (shun) e_lo = s.kv - s.n + (r0 + rows - 1) / a.G - a.window;
                     }
                 }
-                // the warp's rows into shared memory as they are, half a row a thread (the products so far are all done)
-                {
-                    const int r = wr + (lane >> 1), row0 = seg->row0, row = row0 + 128 * g + r;
-                    const bool live = row < seg->n_rows;
-                    const int token = (live ? row : row0) / a.G, head = seg->h * a.G + (live ? row : row0) % a.G;
-                    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(seg->q0 + token) * a.q_row + (long long)head * a.q_head;
-                    unsigned char* dst = smem + C::kOffQ + g * C::kTile + r * 128;
-                    constexpr int N = D / 16;
-                    const int i0 = (lane & 1) * N;
-                    uint4 w[N];
-#pragma unroll
-                    for (int i = 0; i < N; ++i) w[i] = live ? *reinterpret_cast<const uint4*>(src + 8 * (i0 + i)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) *reinterpret_cast<uint4*>(dst + ((i0 + i) >> 3) * 16384 + ((((i0 + i) & 7) ^ (r & 7)) << 4)) = w[i];
-                }
-                fence_async_smem();
-                arrive_w(bar(QREADY + g));
-
                 float2 nm[2], l_run[2];               // minus the row's reference, twice; its sum over even and odd keys
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
@@ -597,7 +605,12 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                     tc_fence_after();
                     if (!rows_here) {                 // rows behind the last one: what P holds for them reaches no output
                         arrive_w(bar(SCEMPTY + sc));
-                        if (C::kOwnP) arrive_w(bar(SEMPTY + g));
+                        if (C::kOwnP) {
+                            arrive_w(bar(SEMPTY + g));
+                            // not before the weights of the tile before have been taken: the others may still be writing those,
+                            // and this arrival would count for them
+                            if (!first && !wait_w(bar(PVDONE + g), (s_run - 1) & 1)) { ok = false; break; }
+                        }
                         arrive_w(bar(PFULL + g));
                         ++s_run;
                         first = false;
@@ -631,15 +644,14 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                         tc_wait_st();
                     }
                     bool pv_done = first || !C::kOwnP;       // without columns of its own, P's S came behind the last PV
-                    float x[kBW / 2];                 // [4 (key / 8) + 2 slot + column]
-                    ld_scores(tmem_S + kBN - kBW, x);
                     // Blocks of kBW keys, highest first (P may lie on the S of the blocks before).  The loop stays rolled, and
                     // nothing in it waits for a maximum: a weight's exponent is taken against the row's reference, and only when
                     // one passes 2^15 -- or the row has no reference yet -- does the warp turn aside to move it.
 #pragma unroll 1
                     for (int cb = kBN / kBW - 1; cb >= 0; --cb) {
                         const float* sk = sa + kBW * cb;
-                        float z[kBW / 2];
+                        float z[kBW / 2];             // [4 (key / 8) + 2 slot + column]
+                        ld_scores(tmem_S + kBW * cb, z);   // (four warps a scheduler cover the wait; a block ahead costs 16 registers)
                         tc_wait_ld();
 #pragma unroll
                         for (int w = 0; w < kBW / 8; ++w) {
@@ -647,7 +659,7 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
 #pragma unroll
                             for (int q = 0; q < 2; ++q) {
                                 const int at = 4 * w + 2 * q;
-                                const float2 t = __ffma2_rn(make_float2(x[at], x[at + 1]), ka, __fadd2_rn(kb, nm[q]));
+                                const float2 t = __ffma2_rn(make_float2(z[at], z[at + 1]), ka, __fadd2_rn(kb, nm[q]));
                                 z[at] = t.x;
                                 z[at + 1] = t.y;
                             }
@@ -661,20 +673,19 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                         if (__builtin_expect(__any_sync(0xffffffffu, fmaxf(t0, t1) > kMoveMax), 0)) {
                             // Move the references of the rows that outgrew theirs to the largest exponent of the block, and scale
                             // what was summed against the old ones: l, O, and the blocks of P that this tile already has.
-                            float y[kBW / 2], f[2];                    // the scores again: z lost them to a reference of -1e30
-                            ld_scores(tmem_S + kBW * cb, y);
+                            ld_scores(tmem_S + kBW * cb, z);           // the scores again: a reference of -1e30 has swallowed them
                             tc_wait_ld();
-                            float top[2] = {-INFINITY, -INFINITY};
+                            float top[2] = {-INFINITY, -INFINITY}, f[2];
 #pragma unroll
                             for (int w = 0; w < kBW / 8; ++w) {
                                 const float2 ka = *reinterpret_cast<const float2*>(sk + 8 * w), kb = *reinterpret_cast<const float2*>(sk + kBN + 8 * w);
 #pragma unroll
                                 for (int q = 0; q < 2; ++q) {
                                     const int at = 4 * w + 2 * q;
-                                    const float2 t = __ffma2_rn(make_float2(y[at], y[at + 1]), ka, kb);
-                                    y[at] = z[at] == -INFINITY ? -INFINITY : t.x;
-                                    y[at + 1] = z[at + 1] == -INFINITY ? -INFINITY : t.y;
-                                    top[q] = fmaxf(top[q], fmaxf(y[at], y[at + 1]));
+                                    const float2 t = __ffma2_rn(make_float2(z[at], z[at + 1]), ka, kb);
+                                    z[at] = t.x;
+                                    z[at + 1] = t.y;
+                                    top[q] = fmaxf(top[q], fmaxf(t.x, t.y));
                                 }
                             }
 #pragma unroll
@@ -684,13 +695,11 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                                 top[q] = ceilf(fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], 2)));
                                 const bool move = top[q] + nm[q].x > kMoveMax;
                                 f[q] = !move ? 1.0f : nm[q].x == -kNoReference ? 0.0f : ex2(-nm[q].x - top[q]);
-                                if (move) {
-                                    nm[q] = make_float2(-top[q], -top[q]);
+                                if (move) nm[q] = make_float2(-top[q], -top[q]);
 #pragma unroll
-                                    for (int w = 0; w < kBW / 8; ++w) {
-                                        z[4 * w + 2 * q] = y[4 * w + 2 * q] - top[q];
-                                        z[4 * w + 2 * q + 1] = y[4 * w + 2 * q + 1] - top[q];
-                                    }
+                                for (int w = 0; w < kBW / 8; ++w) {
+                                    z[4 * w + 2 * q] += nm[q].x;
+                                    z[4 * w + 2 * q + 1] += nm[q].x;
                                 }
                                 l_run[q] = __fmul2_rn(l_run[q], make_float2(f[q], f[q]));
                             }
@@ -724,9 +733,7 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                             tc_wait_st();
                             tc_fence_before();
                         }
-                        if (cb > 0) {                 // the next block's scores, under this one's exponentials
-                            ld_scores(tmem_S + kBW * (cb - 1), x);
-                        } else if (C::kOwnP) {        // all scores have left: the next ones may overwrite these columns
+                        if (C::kOwnP && cb == 0) {    // all scores have left: the next ones may overwrite these columns
                             tc_fence_before();
                             arrive_w(bar(SEMPTY + g));
                         }
@@ -761,6 +768,8 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                     first = false;
                 }
                 if (!ok) break;
+                // the next segment's queries first: its first scores are then computed under what follows
+                if (!load_q(n_seg + 1)) break;
                 // ---- the segment's result: output rows, or partial ones ----
                 if (!first) {
                     if (!wait_w(bar(PVDONE + g), (s_run - 1) & 1)) break;
@@ -804,7 +813,7 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                         }
                 }
                 tc_fence_before();
-                arrive_w(bar(SEGEMPTY + sst));
+                arrive_w(bar(SEGEMPTY + n_seg % kSegStages));
             }
         }
     }
