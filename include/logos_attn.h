@@ -470,7 +470,7 @@ int logos_qk_norm_rope_bwd(logos_ctx* ctx, int dtype, const void* Q, const void*
 typedef struct {
     int8_t *k, *v;               /* [pages][H][page_size][DH], 16-byte aligned      */
     float *k_scale, *v_scale;    /* [pages][H][page_size], 16-byte aligned          */
-    int pages, page_size;        /* page_size 16, 32, 64 or 128                     */
+    int pages, page_size;        /* page_size 16, 32, 64 or 128; at most 2^31 - 1 rows (pages x H x page_size) */
     int H, DH;                   /* key/value heads; DH 64 or 128                   */
 } logos_paged_cache;
 /* The new tokens of a batch of sequences.  Sequence b owns rows [cu_q[b], cu_q[b+1]) of the token tensors; they stand

@@ -47,9 +47,10 @@ __host__ __device__ __forceinline__ int paged_page(const PagedArgs& a, int b, in
     return (unsigned)page < (unsigned)a.pages ? page : -1;
 }
 
-// first row of head h in a page: row r of it has its DH bytes at (that + r) * DH and its scale at that + r
-__host__ __device__ __forceinline__ size_t paged_row(const PagedArgs& a, int page, int h) {
-    return ((size_t)page * a.H + h) << a.page_shift;
+// First row of head h in a page: row r of it has its DH bytes at (that + r) * DH and its scale at that + r.  Rows fit 32
+// bits (paged_check; a row takes 136 bytes at least), their byte offsets do not: widen before the multiplication.
+__host__ __device__ __forceinline__ uint32_t paged_row(const PagedArgs& a, int page, int h) {
+    return ((uint32_t)page * (uint32_t)a.H + (uint32_t)h) << a.page_shift;
 }
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {

@@ -143,8 +143,8 @@ paged_split_kernel(const __grid_constant__ SplitArgs a) {
 #pragma unroll
             for (int j = 0; j < SUB; ++j) {
                 const int page = max(__shfl_sync(0xffffffffu, my_page, (it * SUB + j) & 31), 0);
-                const size_t row = paged_row(a.p, page, h) + ((key + 16 * j) & ((1 << a.p.page_shift) - 1));
-                const int8_t *k = a.p.k + row * D + 16 * lane, *v = a.p.v + row * D + 16 * lane;
+                const uint32_t row = paged_row(a.p, page, h) + ((key + 16 * j) & ((1 << a.p.page_shift) - 1));
+                const int8_t *k = a.p.k + (size_t)row * D + 16 * lane, *v = a.p.v + (size_t)row * D + 16 * lane;
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i) {
                     cp_async16(dst + 16 * j * D + 512 * i, k + 512 * i);

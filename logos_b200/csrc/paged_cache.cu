@@ -228,6 +228,8 @@ int paged_check(logos_ctx* ctx, const char* what, const logos_paged_cache* c, co
     if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
         return fail(ctx, LOGOS_ERR_UNSUPPORTED, "%s: page_size %d (16, 32, 64 or 128)", what, c->page_size);
     if (c->DH != 64 && c->DH != 128) return fail(ctx, LOGOS_ERR_UNSUPPORTED, "%s: DH = %d (64 or 128)", what, c->DH);
+    if ((int64_t)c->pages * c->H * c->page_size > 0x7fffffffLL)
+        return fail(ctx, LOGOS_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows in a cache (pages x H x page_size)", what);
     if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_scale) || !aligned16(c->v_scale))
         return fail(ctx, LOGOS_ERR_ALIGNMENT, "%s: the cache must be 16-byte aligned", what);
     if (b->B < 0 || b->rows < 0 || b->max_q < 0 || b->max_kv < 0 || b->max_pages < 0 || b->B > 65535 ||

@@ -448,7 +448,7 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                         if (n % (16 * PPT) == 0 && n > 0) { pg_last = pg; pg = checked(pg_next); pg_next = entries_from(i + 16); ++group; }
                         const int key = key_first + i * kBN + PR * blk;
                         const int page = max(__shfl_sync(0xffffffffu, pg, 2 * (i & 15) + (PR * blk >> 4)), 0);
-                        const int8_t* at = src + (paged_row(a.p, page, sh) + (key & page_mask) + r16) * D + 16 * c16;
+                        const int8_t* at = src + (size_t)(paged_row(a.p, page, sh) + (key & page_mask) + r16) * D + 16 * c16;
 #pragma unroll
                         for (int u = 0; u < NP; ++u) cp_async16(raw_addr + slot_in * 1024 + u * 512, at + u * RI * D);
                         slot_in = slot_in + 1 == C::kDepth ? 0 : slot_in + 1;
@@ -462,7 +462,7 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                     const int d = (i >> 4) - group;
                     const int page = __shfl_sync(0xffffffffu, d > 0 ? pg_next : d < 0 ? pg_last : pg, 2 * (i & 15) + (lane >> 4));
                     there = (unsigned)page < (unsigned)a.p.pages && key < end;
-                    const size_t row = paged_row(a.p, there ? page : 0, sh) + (key & page_mask);
+                    const uint32_t row = paged_row(a.p, there ? page : 0, sh) + (key & page_mask);
                     ks = __ldg(a.p.ks + row);
                     vs = __ldg(a.p.vs + row);
                 };

@@ -54,6 +54,7 @@ int main() {
         c.H = 0; EXPECT(call(c, batch), LOGOS_ERR_INVALID_ARG); c = cache;
         c.page_size = 48; EXPECT(call(c, batch), LOGOS_ERR_UNSUPPORTED); c = cache;
         c.page_size = 0; EXPECT(call(c, batch), LOGOS_ERR_UNSUPPORTED); c = cache;
+        c.pages = INT_MAX; EXPECT(call(c, batch), LOGOS_ERR_UNSUPPORTED); c = cache;
         c.DH = 96; EXPECT(call(c, batch), LOGOS_ERR_UNSUPPORTED); c = cache;
         c.v += 8; EXPECT(call(c, batch), LOGOS_ERR_ALIGNMENT); c = cache;
         logos_paged_batch b = batch;
@@ -163,7 +164,7 @@ int main() {
                 const int page = logos::paged_page(a, i, pos);
                 if (page < 0) { if (table[at] >= 0 && table[at] < c.pages) ++failures; continue; }
                 ++pages_in;
-                const size_t row = logos::paged_row(a, page, c.H - 1) + (pos & (c.page_size - 1));
+                const size_t row = (size_t)logos::paged_row(a, page, c.H - 1) + (pos & (c.page_size - 1));
                 if (row >= (size_t)c.pages * c.H * c.page_size) ++failures;
             }
         }
