@@ -103,14 +103,14 @@ __device__ __forceinline__ void ld_scores(uint32_t taddr, float (&x)[kBW / 2]) {
 template <int D> struct Shape {
     static constexpr int kTile = kBN * D * 2;                 // one FP16 tile of 128 rows
     static constexpr int kStages = D == 64 ? 3 : 2;           // K tiles
-    static constexpr int kStagesV = D == 64 ? 3 : 2;          // V tiles
+    static constexpr int kStagesV = D == 64 ? 3 : 1;          // V tiles: wanted a softmax later, and the space goes to the fetches
     static constexpr bool kOwnP = D == 64;                    // P has TMEM columns of its own
     static constexpr int kOffQ = 0, kOffK = kOffQ + 2 * kTile, kOffV = kOffK + kStages * kTile;
     static constexpr int kOffScale = kOffV + kStagesV * kTile; // kScaleStages x {a, b, 1/vs: 128 floats each, 4 words of landmarks}
     static constexpr int kScaleBytes = 3 * kBN * 4 + 16;
-    static constexpr int kDepth = D == 64 ? 4 : 3;            // pieces of 1 KiB a converting warp has in flight
+    static constexpr int kRaw = 32 * D;                       // bytes of a converting warp's share of a tile: the fetches run one tile ahead
     static constexpr int kOffRaw = kOffScale + kScaleStages * kScaleBytes;
-    static constexpr int kOffSeg = kOffRaw + 8 * kDepth * 1024;
+    static constexpr int kOffSeg = kOffRaw + 8 * kRaw;
     static constexpr int kOffBar = kOffSeg + kSegStages * 64;
     static constexpr int kNumBars = 2 * (kStages + kStagesV) + 2 * kScaleStages + 2 * kSegStages + 5 * 2 + 1;
     static constexpr int kOffScan = kOffBar + kNumBars * 8;
@@ -399,7 +399,8 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
         if (work) {
             // ================= K (warps 16-19) and V (20-23) to 16 bits =================
             // A warp takes 32 rows of every tile as pieces of 1 KiB (16 or 8 keys), which never cross a page.  A piece's bytes wait
-            // in shared memory, each where the thread that fetched it will read it (no barrier), kDepth pieces in flight.
+            // in shared memory, each where the thread that fetched it will read it (no barrier); a piece that has been converted
+            // makes room for the same piece of the next tile.
             constexpr int LR = D / 16, RI = 32 / LR;                 // lanes of a row, rows of a load
             constexpr int PR = 1024 / D, NP = PR / RI, PPT = 32 / PR;   // rows and loads of a piece, pieces of the warp's share of a tile
             const bool is_v = warp >= kConvWarp + 4;
@@ -410,7 +411,7 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
             auto wait_w = [&](uint32_t bb, uint32_t parity) { return wait_warp(bb, parity, abort_flag); };
             auto arrive_w = [&](uint32_t bb) { __syncwarp(); if (lane == 0) mbar_arrive(bb); };
             const int c16 = lane % LR, r16 = lane / LR;              // 16 channels, first row of a piece
-            unsigned char* raw = smem + C::kOffRaw + (warp - kConvWarp) * (C::kDepth * 1024) + lane * 16;
+            unsigned char* raw = smem + C::kOffRaw + (warp - kConvWarp) * C::kRaw + lane * 16;
             const uint32_t raw_addr = smem_u32(raw);
             const int page_mask = (1 << a.p.page_shift) - 1;
             const int ch = 2 * (c16 & 3);
@@ -436,39 +437,42 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                     report_batch(a.p.status, sb, true);
                     return -1;
                 };
-                int pg = checked(entries_from(0)), pg_next = entries_from(16), pg_last = pg, group = 0;   // group: 16 tiles that pg is for
+                int pg = checked(entries_from(0)), pg_next = entries_from(16);
                 float ks = 0.0f, vs = 0.0f;                          // the scales of this thread's key of the tile
                 bool there = false;
-                int slot_in = 0, slot_out = 0;
-                // fetch piece n of the segment; with a tile's first piece also its scales.  A page that is not there is read as
-                // page 0: its keys weigh nothing, and no load waits for a test.
-                auto fetch = [&](int n) {
-                    if (n < PPT * n_iter) {
-                        const int i = n / PPT, blk = n % PPT;
-                        if (n % (16 * PPT) == 0 && n > 0) { pg_last = pg; pg = checked(pg_next); pg_next = entries_from(i + 16); ++group; }
-                        const int key = key_first + i * kBN + PR * blk;
-                        const int page = max(__shfl_sync(0xffffffffu, pg, 2 * (i & 15) + (PR * blk >> 4)), 0);
-                        const int8_t* at = src + (size_t)(paged_row(a.p, page, sh) + (key & page_mask) + r16) * D + 16 * c16;
+                // Where the thread's first bytes of the two 16-key halves of its share of tile i lie.  A page that is not there is read
+                // as page 0: its keys weigh nothing, and no load waits for a test.
+                const int8_t* at[2];
+                auto locate = [&](int i) {
+                    if ((i & 15) == 0 && i > 0) { pg = checked(pg_next); pg_next = entries_from(i + 16); }
+                    const int key = key_first + i * kBN;
 #pragma unroll
-                        for (int u = 0; u < NP; ++u) cp_async16(raw_addr + slot_in * 1024 + u * 512, at + u * RI * D);
-                        slot_in = slot_in + 1 == C::kDepth ? 0 : slot_in + 1;
+                    for (int j = 0; j < 2; ++j) {
+                        const int page = max(__shfl_sync(0xffffffffu, pg, 2 * (i & 15) + j), 0);
+                        at[j] = src + (size_t)(paged_row(a.p, page, sh) + ((key + 16 * j) & page_mask) + r16) * D + 16 * c16;
                     }
-                    cp_async_commit();
+                };
+                auto fetch = [&](int blk) {                          // piece blk of the located tile
+#pragma unroll
+                    for (int u = 0; u < NP; ++u)
+                        cp_async16(raw_addr + blk * 1024 + u * 512, at[PR * blk >> 4] + ((PR * blk & 15) + u * RI) * D);
                 };
                 auto fetch_scales = [&](int i) {
                     if (is_v || i >= n_iter) return;
                     const int key = key_first + i * kBN + lane;
-                    // (the fetches are up to kDepth - 1 pieces ahead of this tile, or just short of it)
-                    const int d = (i >> 4) - group;
-                    const int page = __shfl_sync(0xffffffffu, d > 0 ? pg_next : d < 0 ? pg_last : pg, 2 * (i & 15) + (lane >> 4));
+                    const int page = __shfl_sync(0xffffffffu, pg, 2 * (i & 15) + (lane >> 4));
                     there = (unsigned)page < (unsigned)a.p.pages && key < end;
                     const uint32_t row = paged_row(a.p, there ? page : 0, sh) + (key & page_mask);
                     ks = __ldg(a.p.ks + row);
                     vs = __ldg(a.p.vs + row);
                 };
+                locate(0);
                 fetch_scales(0);
-#pragma unroll 1
-                for (int n = 0; n < C::kDepth - 1; ++n) fetch(n);
+#pragma unroll
+                for (int blk = 0; blk < PPT; ++blk) {
+                    fetch(blk);
+                    cp_async_commit();
+                }
                 for (int i = 0; ok && i < n_iter; ++i, ++n_t) {
                     if (!is_v) {
                         const int sc = n_t % kScaleStages;
@@ -485,17 +489,18 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                             if (lane == 0) reinterpret_cast<uint32_t*>(sa - w32 + 3 * kBN)[part] = m;
                         }
                         arrive_w(bar(SCFULL + sc));
+                    }
+                    if (i + 1 < n_iter) {
+                        locate(i + 1);
                         fetch_scales(i + 1);
                     }
                     const int depth = is_v ? SV : ST, st = n_t % depth;
                     if (n_t >= depth && !wait_w(bar(EMPTY + st), ((n_t / depth) - 1) & 1)) { ok = false; break; }
                     unsigned char* tile = tiles + st * C::kTile + (c16 >> 2) * 16384 + (w32 + r16) * 128;
-#pragma unroll 1
+#pragma unroll
                     for (int blk = 0; blk < PPT; ++blk) {
-                        fetch(PPT * i + blk + C::kDepth - 1);
-                        cp_async_wait<C::kDepth - 1>();
-                        const unsigned char* in = raw + slot_out * 1024;
-                        slot_out = slot_out + 1 == C::kDepth ? 0 : slot_out + 1;
+                        cp_async_wait<PPT - 1>();
+                        const unsigned char* in = raw + blk * 1024;
                         uint4 xs[NP];
 #pragma unroll
                         for (int u = 0; u < NP; ++u) xs[u] = *reinterpret_cast<const uint4*>(in + u * 512);
@@ -516,6 +521,8 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                             *reinterpret_cast<uint4*>(row + ((ch ^ sw) << 4)) = y0;
                             *reinterpret_cast<uint4*>(row + (((ch + 1) ^ sw) << 4)) = y1;
                         }
+                        if (i + 1 < n_iter) fetch(blk);
+                        cp_async_commit();
                     }
                     fence_async_smem();
                     arrive_w(bar(FULL + st));
@@ -644,10 +651,10 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
                         tc_wait_st();
                     }
                     bool pv_done = first || !C::kOwnP;       // without columns of its own, P's S came behind the last PV
-                    // Blocks of kBW keys, highest first (P may lie on the S of the blocks before).  The loop stays rolled, and
-                    // nothing in it waits for a maximum: a weight's exponent is taken against the row's reference, and only when
-                    // one passes 2^15 -- or the row has no reference yet -- does the warp turn aside to move it.
-#pragma unroll 1
+                    // Blocks of kBW keys, highest first (P may lie on the S of the blocks before).  Nothing in the loop waits for a
+                    // maximum: a weight's exponent is taken against the row's reference, and only when one passes 2^15 -- or the
+                    // row has no reference yet -- does the warp turn aside to move it.
+#pragma unroll
                     for (int cb = kBN / kBW - 1; cb >= 0; --cb) {
                         const float* sk = sa + kBW * cb;
                         float z[kBW / 2];             // [4 (key / 8) + 2 slot + column]
