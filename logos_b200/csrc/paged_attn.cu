@@ -32,7 +32,10 @@ constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = 32 * kSplitWarps;
 constexpr int kStages = 2;                       // blocks in a warp's ring
 constexpr int kSpan = 2048;                      // keys whose pages a warp's lanes hold, one 16-key block each
-constexpr int kFewRows = 32;                     // query rows per head up to which a sequence is this kernel's
+// Query rows per head up to which a sequence is this kernel's.  It reads the keys once per 16 rows (from L2 after the first),
+// the other once per 256 with a longer start.  8 heads over 4000 tokens, this kernel / the other, us: one sequence, 64 rows
+// 21 / 43 (DH 64), 34 / 48 (DH 128); 16 sequences 81 / 101 and 133 / 122; 128 rows 29 / 43, 47 / 50; 140 / 103, 230 / 126.
+constexpr int kFewRows = 64;
 constexpr int kSplitCounters = (int)(kWorkspaceCounterBytes / sizeof(int));
 
 struct SplitArgs {

@@ -43,7 +43,7 @@ constexpr int kSegReaders = kPlanWarp;       // warps 0 ... 25 read every segmen
 constexpr int kItemCost = 4;                  // what an item costs beside its tiles (queries in, pipeline filled, rows out), in tiles
 constexpr float kLeastFactor = 1e-37f;
 constexpr float kNoReference = -1e30f;       // reference of a row that has seen no key: any visible key lies above it
-constexpr int kJoinRows = 32;                // rows a CTA of the join takes
+constexpr int kJoinRows = 8;                 // rows a CTA of the join takes, a warp each
 
 // One poll of a barrier, asleep for up to 20 us; a waiting warp that polls by itself takes issue slots from the working ones.
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
@@ -838,7 +838,7 @@ paged_chunk_kernel(const __grid_constant__ ChunkArgs a) {
     }
 }
 
-// Joins the items that were cut: CTA (c, y) takes rows [32 y, 32 y + 32) of the item that begins in CTA c of the chunk
+// Joins the items that were cut: CTA (c, y) takes rows [8 y, 8 y + 8) of the item that begins in CTA c of the chunk
 // kernel.  A warp per row; the parts follow one another in the order of the keys.
 template <int D>
 __global__ void __launch_bounds__(256)

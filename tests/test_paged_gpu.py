@@ -197,6 +197,8 @@ ATTEND = [  # n_q, n_kv, H, G, D, page, window, stride, causal, layout, dtype
     ([129, 513], [129, 4000], 1, 4, 128, 128, 0, 0, True, "tokens", "fp16"),
     ([600], [3000], 1, 2, 64, 32, 200, 0, True, "tokens", "bf16"),
     ([385], [1100], 1, 1, 128, 16, 90, 33, True, "heads", "bf16"),
+    ([64, 65, 33], [700, 700, 33], 2, 1, 128, 32, 0, 0, True, "tokens", "fp16"),   # either side of the two kernels' border
+    ([32, 33], [300, 4000], 2, 2, 64, 64, 0, 0, True, "heads", "bf16"),
     ([1000], [2000], 2, 1, 64, 64, 0, 0, True, "tokens", "bf16"),      # warps of the last row tile without a row
     ([300, 33, 140], [3000, 5000, 140], 4, 1, 64, 16, 0, 0, True, "heads", "fp16"),
 ]
