@@ -430,8 +430,8 @@ int logos_gemm_f32(logos_ctx* ctx, const float* A, int lda, int64_t strideA, con
  *   n_i = x_i w_i / sqrt(mean(x^2) + eps)
  *   pair k of the first `dims` channels, (a, b) = (k, k + dims/2) or, interleaved, (2k, 2k + 1), angle p inv_freq[k]:
  *   y_a = n_a cos - n_b sin,   y_b = n_b cos + n_a sin;   channels from `dims` on: y_i = n_i.
- * fp32 arithmetic, one rounding at the end.  The angle is reduced exactly (position times a 64-bit fixed-point
- * number of turns), so it is as good at position 2^31 - 1 as at 1. */
+ * fp32 arithmetic, one rounding at the end.  The angle is reduced in integers (position times a 64-bit fixed-point
+ * number of turns, made from the double): for frequencies up to 1 it is right to 2^-22 of a turn at position 2^31 - 1. */
 #define LOGOS_ROPE_MAX_PAIRS 64
 typedef struct {
     int dims;          /* rotated channels: 0 (none) ... DH, a multiple of 16 */

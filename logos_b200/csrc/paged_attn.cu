@@ -15,7 +15,7 @@
 // never moves between threads.  The order of the channels inside a product is free, so a thread's share of a K row is
 // 16 consecutive bytes and its share of a V row DH / 8.  Blocks of 32 keys and their scales come by
 // cp.async into a ring of each warp's own, kStages blocks in flight and no registers spent on them.  (By cp.async.bulk, one
-// lane for all, it took 80 instructions more a block, for the operands of its eight copies: 237 us where this takes 197, 64 sequences x
+// lane for all, it took 80 instructions more a block, for the operands of its eight copies: 237 us where this took 197, 64 sequences x
 // 16 heads x 8192 tokens.)  (tcgen05 needs 128 rows to be busy and its operands in shared memory; here a head has 1 to 16.)
 // int8 -> FP16 costs five instructions for four values: bytes biased to unsigned, spliced under the exponent of 1024
 // and the bias subtracted.
@@ -23,6 +23,9 @@
 // A CTA takes one sequence, head, tile of 8 or 16 rows and one chunk of the keys; its four warps take the chunk's
 // blocks in turn, each with its own running maximum, and join in shared memory.  Chunks join through the workspace:
 // the last CTA to arrive sums the partial results in the order of the chunks.
+//
+// Measured: one token each of 64 sequences x 16 heads x 8192 tokens, DH 64, 194 us = 5.9 TB/s (0.90 of a plain copy);
+// 4 sequences of 1,300 to 9,000 tokens, 32 heads over 8, DH 128, 21 us, 5 of them the join, at 3 CTAs per SM unevenly filled.
 #include "paged.cuh"
 
 namespace logos {

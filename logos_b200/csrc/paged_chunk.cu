@@ -7,8 +7,16 @@
 //
 // What bounds it: per 256 rows x 128 keys the exponentials (16 a clock and SM: 2048 clocks) and the products
 // (M128 N128 K16 in 67 clocks, N64 in 57 to 63: 1500 clocks at DH 64, 2150 at DH 128); the cache itself is read once
-// per 256 rows and comes from L2 after the first.  So the threads' chain per tile decides, and everything that is not
-// softmax is taken off the softmax threads.
+// per 256 rows and comes from L2 after the first.  Measured it is the threads' instructions: some 13,400 of a warp per
+// 256 x 128 scores at DH 128, 0.56 a clock and scheduler.  2048 tokens over 16,384, 32 heads over 8, DH 128: 756 us =
+// 680 TFLOP/s (0.42 of a plain product), 14 us more for the join.  Hence:
+//  - 16 softmax warps of 16 rows, each thread 32 keys of two rows through 16x256-bit TMEM loads: the three numbers of a key
+//    then cost a quarter of the shared-memory reads that one thread per row makes (a broadcast takes its 128 bytes a
+//    clock like any other read): 1162 -> 1075 us;
+//  - no maximum before the exponentials: a row's reference is the last tile's, and only a weight above 2^kMoveMax makes
+//    the warp take the tile again with a new one: 1075 -> 963;
+//  - the softmax loop without a spill (200 KB of shared memory leave local memory little L1): 920 -> 830;
+//  - pages looked up per tile, rows fetched a tile ahead, everything on warps of its own: 830 -> 763.
 //
 // A CTA (896 threads, one per SM) holds two 128-row tiles of one (sequence, head) -- row r is token r / G, query head
 // r % G of the group, so grouped heads share every K and V tile -- and walks over key tiles of 128.  Roles:

@@ -7,6 +7,10 @@
 // The angle p f is wanted modulo one turn and p goes up to 2^31: the frequency comes as a 64-bit fixed-point number of
 // turns, the product p F wraps modulo 2^64 by itself and its upper word is the fraction of a turn to 2^-32.  (A float
 // product is off by 2^-24 p f radians: useless from p f ~ 10^5 on.)
+//
+// Measured: forward, 65,536 tokens x 32 heads x 64 BF16, 98 us = 5.5 TB/s (0.84 of a plain copy); backward, 16,384 tokens x
+// 40 heads x 128 BF16 with both weights' gradients, 101 us = 5.0 TB/s, the sum of the partial gradients mostly under it;
+// 32 tokens 3 us, which is the launch.
 #include <cmath>
 
 #include "common.cuh"
