@@ -24,14 +24,13 @@ _STRIDES: dict = {}
 
 
 def _strides(row, head):
-    """Address of a logos_row_strides with these values."""
+    """A logos_row_strides with these values, by reference (which keeps it alive when the store is emptied)."""
     got = _STRIDES.get((row, head))
     if got is None:
         if len(_STRIDES) >= 4096:
             _STRIDES.clear()
-        desc = L.RowStrides(row, head)
-        got = _STRIDES[(row, head)] = (C.addressof(desc), desc)
-    return got[0]
+        got = _STRIDES[(row, head)] = C.byref(L.RowStrides(row, head))
+    return got
 
 
 class Engine:
@@ -252,7 +251,7 @@ class Engine:
     # A serving loop makes these calls once per layer and token, so the checks are few and cheap, pointers travel as
     # plain integers and the descriptors were laid out when their handles were made.
     def _view(self, what, t, rows, heads, dh, dtype):
-        """Address of the strides of `t`, a [rows, heads, DH] view with contiguous channels on this device."""
+        """The strides of `t`, a [rows, heads, DH] view with contiguous channels on this device."""
         if t.shape != (rows, heads, dh) or t.dtype != dtype:
             raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)} where {dtype} {(rows, heads, dh)} is needed")
         row, head, one = t.stride()
@@ -345,18 +344,19 @@ class Engine:
 
     # ---- paged INT8 KV ---------------------------------------------------------
     def _paged(self, what, cache, batch, rows):
+        """The batch's descriptor for token tensors of `rows` rows."""
         if cache.device_index != self.device or batch.device_index != self.device:
             raise ValueError(f"{what}: cache on device {cache.device_index}, batch on {batch.device_index}, the engine on {self.device}")
-        batch.desc.rows = rows
+        return batch.over(rows)
 
     def paged_append(self, K, V, cache, batch):
         """The batch's new K and V rows ([rows, H, DH], any row and head strides) quantised into their pages, a scale
-        per row.  rows may exceed the batch's last row: those are not read."""
+        per row.  rows may exceed the batch's last row: those are not used."""
         what, rows, dtype = "paged_append", K.shape[0], K.dtype
         sk = self._view(what, K, rows, cache.heads, cache.dh, dtype)
         sv = self._view(what, V, rows, cache.heads, cache.dh, dtype)
-        self._paged(what, cache, batch, rows)
-        rc = self.lib.logos_paged_append(self.h, _DT.get(dtype, -1), K.data_ptr(), V.data_ptr(), sk, sv, cache.address, batch.address)
+        desc = self._paged(what, cache, batch, rows)
+        rc = self.lib.logos_paged_append(self.h, _DT.get(dtype, -1), K.data_ptr(), V.data_ptr(), sk, sv, cache.address, desc)
         if rc:
             self._check(rc)
 
@@ -366,8 +366,8 @@ class Engine:
         what, rows, dtype = "paged_read", out_k.shape[0], out_k.dtype
         sk = self._view(what, out_k, rows, cache.heads, cache.dh, dtype)
         sv = self._view(what, out_v, rows, cache.heads, cache.dh, dtype)
-        self._paged(what, cache, batch, rows)
-        rc = self.lib.logos_paged_read(self.h, _DT.get(dtype, -1), cache.address, batch.address, out_k.data_ptr(), out_v.data_ptr(), sk, sv)
+        desc = self._paged(what, cache, batch, rows)
+        rc = self.lib.logos_paged_read(self.h, _DT.get(dtype, -1), cache.address, desc, out_k.data_ptr(), out_v.data_ptr(), sk, sv)
         if rc:
             self._check(rc)
         return out_k, out_v
@@ -383,8 +383,8 @@ class Engine:
             out = torch.empty((rows, Hq, DH), dtype=dtype, device=Q.device)
         sq = self._view(what, Q, rows, Hq, cache.dh, dtype)
         so = self._view(what, out, rows, Hq, DH, dtype)
-        self._paged(what, cache, batch, rows)
-        args = (self.h, _DT.get(dtype, -1), Q.data_ptr(), cache.address, batch.address, Hq, C.byref(params), out.data_ptr(), sq, so)
+        desc = self._paged(what, cache, batch, rows)
+        args = (self.h, _DT.get(dtype, -1), Q.data_ptr(), cache.address, desc, Hq, C.byref(params), out.data_ptr(), sq, so)
         rc = self.lib.logos_paged_attention(*args)
         if rc == L.ERR_WORKSPACE:
             self.reserve(self.paged_attention_workspace_bytes(cache, batch, rows, Hq))
@@ -394,8 +394,8 @@ class Engine:
         return out
 
     def paged_attention_workspace_bytes(self, cache, batch, rows, Hq):
-        self._paged("paged_attention", cache, batch, rows)
-        return self.lib.logos_paged_attention_workspace_bytes(self.h, cache.address, batch.address, Hq)
+        desc = self._paged("paged_attention", cache, batch, rows)
+        return self.lib.logos_paged_attention_workspace_bytes(self.h, cache.address, desc, Hq)
 
     # ---- Nikhilam INT8 KV ----------------------------------------------------
     def prefill(self, Q, K, V, params: L.Params, k_cache, v_cache, k_scale, v_scale, out_dtype=None, out=None):

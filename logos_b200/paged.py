@@ -97,9 +97,18 @@ class PagedBatch:
             raise ValueError("PagedBatch: tensors on several devices")
         self.cu_q, self.kv_len, self.page_table = cu_q, kv_len, page_table
         self.B, self.max_q, self.max_kv = B, int(max_q), int(max_kv)
-        self.desc = L.PagedBatch(cu_q.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), B, page_table.shape[1], 0,
-                                 self.max_q, self.max_kv)
-        self.address, self.device_index = C.addressof(self.desc), cu_q.get_device()
+        self.device_index = cu_q.get_device()
+        self._over = (-1, None)
+
+    def over(self, rows: int):
+        """logos_paged_batch for token tensors of `rows` rows, by reference.  Another number of rows takes another descriptor:
+        the one that a call on another thread holds stays as it is."""
+        held, desc = self._over
+        if held != rows:
+            desc = C.byref(L.PagedBatch(self.cu_q.data_ptr(), self.kv_len.data_ptr(), self.page_table.data_ptr(), self.B,
+                                        self.page_table.shape[1], rows, self.max_q, self.max_kv))
+            self._over = (rows, desc)
+        return desc
 
     def positions(self, rows: int) -> torch.Tensor:
         """int32 [rows]: the position of every token row (0 for rows behind the last sequence)."""

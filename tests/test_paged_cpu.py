@@ -110,3 +110,16 @@ def test_handles_refuse_what_does_not_fit():
     r = Rope(32, 500.0, True)
     assert r.desc.dims == 32 and r.desc.interleaved == 1 and list(r.desc.inv_freq)[:2] == [1.0, 500.0 ** (-1 / 16)]
     assert L.load_library().logos_status_string(L.ERR_BAD_BATCH) != b"unknown status"
+
+
+def test_descriptors_outlive_the_stores_they_came_from():
+    """A call holds several strides and a batch's descriptor at once, and others may be made meanwhile."""
+    from logos_b200.engine import _strides
+    held = [_strides(3 * i + 64, 128 * i) for i in range(4)]
+    for i in range(10000):
+        _strides(64 * i, 7)
+    assert [(d._obj.row, d._obj.head) for d in held] == [(3 * i + 64, 128 * i) for i in range(4)]
+    batch = PagedBatch(torch.tensor([0, 3], dtype=torch.int32), torch.tensor([10], dtype=torch.int32),
+                       torch.zeros((1, 1), dtype=torch.int32), 3, 10)
+    few, many = batch.over(3), batch.over(9)
+    assert (few._obj.rows, many._obj.rows, batch.over(9)._obj.max_kv) == (3, 9, 10)
