@@ -475,7 +475,7 @@ typedef struct {
 } logos_paged_cache;
 /* The new tokens of a batch of sequences.  Sequence b owns rows [cu_q[b], cu_q[b+1]) of the token tensors; they stand
  * at positions kv_len[b] - n ... kv_len[b] - 1 (n of them); position p lives in row p % page_size of page
- * page_table[b][p / page_size].  Rows from cu_q[B] on are neither read nor written.  The three tables are device
+ * page_table[b][p / page_size].  Rows from cu_q[B] on are neither used nor written.  The three tables are device
  * memory, so that a captured graph replays with new contents; B, rows, max_q and max_kv are host-side bounds that
  * size the launches.  Sequences may share pages that none of them writes in the call; a page row that two sequences
  * write in one call holds the row of either or a mixture of both.
@@ -487,15 +487,15 @@ typedef struct {
     const int32_t* kv_len;       /* [B]: tokens of the sequence, the new ones included */
     const int32_t* page_table;   /* [B][max_pages]; entries behind the last page in use are not read */
     int B, max_pages;
-    int rows;                    /* rows of the token tensors, at least cu_q[B]     */
-    int max_q, max_kv;           /* bounds of a sequence's new tokens and of kv_len; max_kv <= max_pages * page_size */
+    int rows;                    /* rows of the token tensors, at least cu_q[B]; at most 2^30 */
+    int max_q, max_kv;           /* bounds of a sequence's new tokens and of kv_len; max_kv <= max_pages * page_size, 2^30 */
 } logos_paged_batch;
 
 /* Quantises the new tokens' K and V ([rows][H][DH] in `dtype`, F32, BF16 or FP16; strides or NULL) into their pages. */
 int logos_paged_append(logos_ctx* ctx, int dtype, const void* K, const void* V, const logos_row_strides* k_in,
                        const logos_row_strides* v_in, const logos_paged_cache* cache, const logos_paged_batch* batch);
 /* The inverse: the values (float)q * scale that the cache holds for the batch's rows, in `dtype`.  cu_q over whole
- * sequences (n = kv_len) reads all of them out. */
+ * sequences (n = kv_len) reads all of them out.  The outputs may not overlap. */
 int logos_paged_read(logos_ctx* ctx, int dtype, const logos_paged_cache* cache, const logos_paged_batch* batch, void* K,
                      void* V, const logos_row_strides* k_out, const logos_row_strides* v_out);
 /* Attention of the batch's new tokens -- one per sequence, a chunk of a prompt, or both kinds in one call -- over the

@@ -170,6 +170,7 @@ constexpr size_t kWorkspaceCounterBytes = 64 * 1024;
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 
+constexpr int kMostRows = 1 << 30;       // token rows of a call, positions of a sequence
 // strides of a [rows][heads][DH] tensor: every row on a 16-byte boundary; no two rows on one another (an output)
 inline bool rows_aligned(const logos_row_strides& s, size_t esz) {
     return s.row >= 0 && s.head >= 0 && (s.row * esz) % 16 == 0 && (s.head * esz) % 16 == 0;

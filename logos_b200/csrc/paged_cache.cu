@@ -238,6 +238,8 @@ int paged_check(logos_ctx* ctx, const char* what, const logos_paged_cache* c, co
         (int64_t)b->max_kv > (int64_t)b->max_pages * c->page_size || b->max_q > b->max_kv)
         return fail(ctx, LOGOS_ERR_INVALID_ARG, "%s: bad batch (B %d up to 65535, rows %d, max_q %d <= max_kv %d <= %d pages x %d)",
                     what, b->B, b->rows, b->max_q, b->max_kv, b->max_pages, c->page_size);
+    if (b->rows > kMostRows || b->max_kv > kMostRows)        // the kernels round row numbers and positions up in 32 bits
+        return fail(ctx, LOGOS_ERR_UNSUPPORTED, "%s: rows %d, max_kv %d (2^30 at most)", what, b->rows, b->max_kv);
     if (b->B > 0 && (!b->cu_q || !b->kv_len || (b->max_kv > 0 && !b->page_table)))
         return fail(ctx, LOGOS_ERR_INVALID_ARG, "%s: null table", what);
     return LOGOS_OK;

@@ -303,6 +303,7 @@ int qk_norm_rope(logos_ctx* ctx, int dtype, bool bwd, const void* Q, const void*
         return fail(ctx, LOGOS_ERR_INVALID_ARG, "%s: rope dims %d (a multiple of 16 up to DH)", what, rope->dims);
     if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(ctx, LOGOS_ERR_INVALID_ARG, "%s: eps must be finite and not negative", what);
     if (Hq > 1024 || Hk > 1024) return fail(ctx, LOGOS_ERR_UNSUPPORTED, "%s: more than 1024 heads", what);
+    if (rows > kMostRows) return fail(ctx, LOGOS_ERR_UNSUPPORTED, "%s: %d rows (2^30 at most)", what, rows);
     RopeArgs a = {};
     for (int k = 0; k < rope->dims / 2; ++k) {
         const double f = rope->inv_freq[k];

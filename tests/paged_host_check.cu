@@ -58,6 +58,8 @@ int main() {
         c.DH = 96; EXPECT(call(c, batch), LOGOS_ERR_UNSUPPORTED); c = cache;
         c.v += 8; EXPECT(call(c, batch), LOGOS_ERR_ALIGNMENT); c = cache;
         logos_paged_batch b = batch;
+        b.rows = (1 << 30) + 1; EXPECT(call(c, b), LOGOS_ERR_UNSUPPORTED); b = batch;
+        b.max_pages = INT_MAX; b.max_kv = (1 << 30) + 1; EXPECT(call(c, b), LOGOS_ERR_UNSUPPORTED); b = batch;
         b.B = -1; EXPECT(call(c, b), LOGOS_ERR_INVALID_ARG); b = batch;
         b.B = 65536; EXPECT(call(c, b), LOGOS_ERR_INVALID_ARG); b = batch;
         b.max_kv = 257; EXPECT(call(c, b), LOGOS_ERR_INVALID_ARG); b = batch;
@@ -104,6 +106,7 @@ int main() {
     EXPECT(rotate(LOGOS_BF16, nullptr, 1e-6f, 4, 2, 2, 64), LOGOS_ERR_INVALID_ARG);
     EXPECT(rotate(LOGOS_BF16, &rope, 1e-6f, -1, 2, 2, 64), LOGOS_ERR_INVALID_ARG);
     EXPECT(rotate(LOGOS_BF16, &rope, 1e-6f, 4, 0, 0, 64), LOGOS_ERR_INVALID_ARG);
+    EXPECT(rotate(LOGOS_BF16, &rope, 1e-6f, (1 << 30) + 1, 2, 2, 64), LOGOS_ERR_UNSUPPORTED);
     EXPECT(rotate(LOGOS_BF16, &rope, 1e-6f, 4, 2, 2, 80), LOGOS_ERR_UNSUPPORTED);
     EXPECT(rotate(LOGOS_BF16, &rope, 1e-6f, 4, 1025, 2, 64), LOGOS_ERR_UNSUPPORTED);
     EXPECT(rotate(LOGOS_BF16, &rope, -1.0f, 4, 2, 2, 64), LOGOS_ERR_INVALID_ARG);

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from logos_b200 import lib as L
+from logos_b200.engine import Engine
 from logos_b200.paged import PagedBatch, PagedKVCache, PagePool, Rope
 
 pytestmark = pytest.mark.gpu
@@ -201,6 +202,8 @@ ATTEND = [  # n_q, n_kv, H, G, D, page, window, stride, causal, layout, dtype
     ([32, 33], [300, 4000], 2, 2, 64, 64, 0, 0, True, "heads", "bf16"),
     ([1000], [2000], 2, 1, 64, 64, 0, 0, True, "tokens", "bf16"),      # warps of the last row tile without a row
     ([300, 33, 140], [3000, 5000, 140], 4, 1, 64, 16, 0, 0, True, "heads", "fp16"),
+    ([1, 3], [1000, 40], 1, 128, 64, 64, 0, 0, True, "tokens", "bf16"),            # many query heads over one: one token is a chunk
+    ([1, 2, 1], [5000, 2, 1], 1, 71, 128, 16, 300, 9, True, "heads", "fp16"),
 ]
 
 
@@ -491,3 +494,64 @@ def test_refusals(engine):
     engine.paged_append(empty, empty, cache, none)
     assert engine.paged_attention(empty, cache, none, params).shape == empty.shape
     engine.synchronize()
+
+
+@pytest.mark.parametrize("n_q,D,page", [(3, 64, 64), (70, 128, 16)])
+def test_offsets_beyond_32_bits(engine, n_q, D, page):
+    """Pages more than 2^32 bytes into the cache, token tensors whose heads lie more than 2^31 values apart."""
+    H, kv, far = 2, 700, 2 ** 31 + 64
+    pages = 2 ** 32 // (H * page * D) + 200
+    cache = fresh(pages, H, page, D)
+    n = -(-kv // page)
+    table = torch.arange(pages - 1, pages - 1 - n, -1, dtype=torch.int32, device="cuda")[None].contiguous()
+    cu = lambda m: torch.tensor([0, m], dtype=torch.int32, device="cuda")  # noqa: E731
+    held = torch.tensor([kv], dtype=torch.int32, device="cuda")
+    whole, batch = PagedBatch(cu(kv), held, table, kv, kv), PagedBatch(cu(n_q), held, table, n_q, kv)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    store = torch.empty(far + kv * D, dtype=torch.bfloat16, device="cuda")
+    apart = lambda m: store.as_strided((m, H, D), (D, far, 1))  # noqa: E731
+    K, V, Q = (torch.randn((m, H, D), generator=g, device="cuda").bfloat16() for m in (kv, kv, n_q))
+    apart(kv).copy_(K)
+    engine.paged_append(apart(kv), V, cache, whole)
+    k_far, v_far = apart(kv), torch.empty((kv, H, D), dtype=torch.bfloat16, device="cuda")
+    store.zero_()
+    engine.paged_read(cache, whole, k_far, v_far)
+    for got, want in ((k_far, K), (v_far, V)):
+        # half a step of the quantiser and half a step of BF16, each relative to the row's largest value
+        top = want.double().abs().amax(-1, keepdim=True)
+        assert ((got.double() - want.double()).abs() <= (0.5 / 127.5 + 2.0 ** -8) * 1.01 * top).all()
+    params = L.Params.make(D ** -0.5)
+    apart(n_q).copy_(Q)
+    got = engine.paged_attention(apart(n_q), cache, batch, params)
+    out = engine.paged_attention(Q, cache, batch, params, out=apart(n_q))
+    engine.synchronize()
+    check_attention(got, Q, cache, batch, params, page)
+    assert torch.equal(out, got)
+    pos = torch.arange(n_q, dtype=torch.int32, device="cuda")
+    apart(n_q).copy_(Q)
+    want, _ = engine.qk_norm_rope(Q, None, None, None, pos, Rope(D))
+    there, _ = engine.qk_norm_rope(apart(n_q), None, None, None, pos, Rope(D), out_q=apart(n_q))
+    assert torch.equal(there, want)
+
+
+@pytest.mark.parametrize("n_q", [1, 90])
+def test_two_contexts_at_once(engine, n_q):
+    """Two engines on streams of their own read one cache at the same time, each with its workspace."""
+    cache, batch, g = filled(engine, [n_q, n_q, 1], [3000, 700, 5000], 2, 64, 32, seed=8)
+    Q = torch.randn((2 * n_q + 1, 4, 64), generator=g, device="cuda").bfloat16()
+    params = L.Params.make(0.125)
+    want = engine.paged_attention(Q, cache, batch, params)
+    engine.synchronize()
+    others = [Engine(0) for _ in range(2)]
+    outs = [[torch.empty_like(Q) for _ in range(10)] for _ in others]
+    for e in others:
+        e.use_stream(torch.cuda.Stream())
+        e.reserve(e.paged_attention_workspace_bytes(cache, batch, Q.shape[0], 4))
+    torch.cuda.synchronize()
+    for i in range(10):
+        for e, o in zip(others, outs):
+            e.paged_attention(Q, cache, batch, params, out=o[i])
+    for e, os_ in zip(others, outs):
+        e.synchronize()
+        assert all(torch.equal(o, want) for o in os_)
+        e.close()
