@@ -64,14 +64,17 @@ class PagedStack:
         requests = [(seq, list(ids)) for seq, ids in requests]
         if not requests or any(not ids for _, ids in requests):
             raise ValueError("PagedStack.step: every request brings at least one token")
+        tokens = [int(t) for _, ids in requests for t in ids]
+        if min(tokens) < 0 or max(tokens) >= self.embed.shape[0]:
+            raise ValueError(f"PagedStack.step: a token outside the vocabulary of {self.embed.shape[0]}")
         longest = max(self.pool.length(seq) + len(ids) for seq, ids in requests)
         if longest > self.cfg.max_seq_len:
             raise ValueError(f"PagedStack.step: {longest} tokens in a sequence, the model takes {self.cfg.max_seq_len}")
         cfg, eng, dev = self.cfg, self.eng, self.embed.device
         batch = self.pool.batch([(seq, len(ids)) for seq, ids in requests], device=dev)
-        rows = sum(len(ids) for _, ids in requests)
+        rows = len(tokens)
         positions = batch.positions(rows)
-        x = self.embed[torch.tensor([t for _, ids in requests for t in ids], dtype=torch.long, device=dev)]
+        x = self.embed[torch.tensor(tokens, dtype=torch.long, device=dev)]
         heads = torch.empty((1, cfg.num_heads, rows, 64), dtype=self.dtype, device=dev)
         for l in range(cfg.num_layers):
             xn = eng.layer_norm(x, self.ln_g[l], self.ln_b[l], 1e-5)

@@ -69,6 +69,20 @@ def test_refusals_without_a_device():
         PagedStack(None, CFG, {}, 4, dtype=torch.float32)
 
 
+def test_a_refused_step_takes_nothing():
+    """Every refusal stands before the pages are taken and before the first kernel."""
+    st = PagedStack(None, CFG, weights(CFG, "cpu"), 4)
+    a, b = st.open(), st.open()
+    for bad in ([(a, [1, CFG.vocab_size])], [(a, [1]), (b, [-1])], [(a, [])], [], [(a, [1]), (a, [2])], [(a, [1] * 701)]):
+        with pytest.raises(ValueError):
+            st.step(bad)
+    with pytest.raises(MemoryError):
+        st.step([(a, [1] * 200), (b, [2] * 100)])
+    with pytest.raises(KeyError):
+        st.step([(a, [1]), (77, [2])])
+    assert st.pool.free_pages == 4 and st.pool.length(a) == st.pool.length(b) == 0
+
+
 @pytest.mark.gpu
 def test_chunks_steps_and_forks(engine):
     w = weights(CFG, "cuda")
