@@ -290,7 +290,9 @@ class Engine:
             sq = self._view(what, Q, rows, hq, DH, dtype)
             if out_q is None:
                 out_q = torch.empty_like(Q)
-            syq = self._view(what, out_q, rows, hq, DH, dtype)
+                syq = _strides(*out_q.stride()[:2])
+            else:
+                syq = self._view(what, out_q, rows, hq, DH, dtype)
             q, yq = Q.data_ptr(), out_q.data_ptr()
         elif out_q is not None:
             raise ValueError(f"{what}: an output without its input")
@@ -299,7 +301,9 @@ class Engine:
             sk = self._view(what, K, rows, hk, DH, dtype)
             if out_k is None:
                 out_k = torch.empty_like(K)
-            syk = self._view(what, out_k, rows, hk, DH, dtype)
+                syk = _strides(*out_k.stride()[:2])
+            else:
+                syk = self._view(what, out_k, rows, hk, DH, dtype)
             k, yk = K.data_ptr(), out_k.data_ptr()
         elif out_k is not None:
             raise ValueError(f"{what}: an output without its input")
@@ -311,29 +315,32 @@ class Engine:
         return out_q, out_k
 
     def qk_norm_rope_bwd(self, Q, K, dQ_out, dK_out, q_weight, k_weight, positions, rope, eps=1e-6):
-        """Gradients (dQ, dK, dq_weight, dk_weight) of qk_norm_rope for the gradients of its outputs; dQ and dK packed in
-        the inputs' type, the weights' in fp32 (None where the weight, or the tensor, is None)."""
+        """Gradients (dQ, dK, dq_weight, dk_weight) of qk_norm_rope for the gradients of its outputs; dQ and dK in
+        the inputs' type and laid out as the inputs are, the weights' in fp32 (None where the weight, or the tensor, is None)."""
         what = "qk_norm_rope_bwd"
         rows, DH, dtype = self._rope_args(what, Q, K, q_weight, k_weight, positions)
         if (Q is None) != (dQ_out is None) or (K is None) != (dK_out is None):
             raise ValueError(f"{what}: a gradient without its tensor, or a tensor without its gradient")
         hq = hk = 0
-        q = k = gq = gk = sq = sk = sgq = sgk = dQ = dK = dwq = dwk = None
+        q = k = gq = gk = wq = wk = sq = sk = sgq = sgk = sdq = sdk = dQ = dK = dwq = dwk = pdq = pdk = pwq = pwk = None
         if Q is not None:
             hq = Q.shape[1]
             sq, sgq = self._view(what, Q, rows, hq, DH, dtype), self._view(what, dQ_out, rows, hq, DH, dtype)
-            q, gq, dQ = Q.data_ptr(), dQ_out.data_ptr(), torch.empty((rows, hq, DH), dtype=dtype, device=Q.device)
+            dQ = torch.empty_like(Q)
+            q, gq, pdq, sdq = Q.data_ptr(), dQ_out.data_ptr(), dQ.data_ptr(), _strides(*dQ.stride()[:2])
         if K is not None:
             hk = K.shape[1]
             sk, sgk = self._view(what, K, rows, hk, DH, dtype), self._view(what, dK_out, rows, hk, DH, dtype)
-            k, gk, dK = K.data_ptr(), dK_out.data_ptr(), torch.empty((rows, hk, DH), dtype=dtype, device=K.device)
+            dK = torch.empty_like(K)
+            k, gk, pdk, sdk = K.data_ptr(), dK_out.data_ptr(), dK.data_ptr(), _strides(*dK.stride()[:2])
         if q_weight is not None:
             dwq = torch.empty_like(q_weight)
+            wq, pwq = q_weight.data_ptr(), dwq.data_ptr()
         if k_weight is not None:
             dwk = torch.empty_like(k_weight)
-        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        args = (self.h, _DT[dtype], q, k, gq, gk, ptr(q_weight), ptr(k_weight), positions.data_ptr(), rope.address, eps, ptr(dQ),
-                ptr(dK), ptr(dwq), ptr(dwk), rows, hq, hk, DH, sq, sk, sgq, sgk, None, None)
+            wk, pwk = k_weight.data_ptr(), dwk.data_ptr()
+        args = (self.h, _DT[dtype], q, k, gq, gk, wq, wk, positions.data_ptr(), rope.address, eps, pdq, pdk, pwq, pwk, rows, hq, hk,
+                DH, sq, sk, sgq, sgk, sdq, sdk)
         rc = self.lib.logos_qk_norm_rope_bwd(*args)
         if rc == L.ERR_WORKSPACE:
             self.reserve(self.lib.logos_qk_norm_rope_bwd_workspace_bytes(DH))
