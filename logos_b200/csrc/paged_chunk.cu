@@ -7,8 +7,9 @@
 //
 // What bounds it: per 256 rows x 128 keys the exponentials (16 a clock and SM: 2048 clocks) and the products
 // (M128 N128 K16 in 67 clocks, N64 in 57 to 63: 1500 clocks at DH 64, 2150 at DH 128); the cache itself is read once
-// per 256 rows and comes from L2 after the first.  Measured it is the threads' instructions: some 13,400 of a warp per
-// 256 x 128 scores at DH 128, 0.56 a clock and scheduler.  2048 tokens over 16,384, 32 heads over 8, DH 128: 756 us =
+// per 256 rows and comes from L2 after the first.  Measured it is the threads: some 13,400 instructions of a warp per
+// 256 x 128 scores at DH 128, issued in 0.45 of a scheduler's clocks; the rest are waits for tensor memory that 16 softmax
+// warps, all that the registers allow, do not cover.  2048 tokens over 16,384, 32 heads over 8, DH 128: 756 us =
 // 680 TFLOP/s (0.42 of a plain product), 14 us more for the join.  Hence:
 //  - 16 softmax warps of 16 rows, each thread 32 keys of two rows through 16x256-bit TMEM loads: the three numbers of a key
 //    then cost a quarter of the shared-memory reads that one thread per row makes (a broadcast takes its 128 bytes a
